@@ -158,19 +158,12 @@ def prepare(case, seed):
     return s
 
 
-_ml = None
-
-
 def _calls():
-    global _ml
-    if _ml is not None:
-        return _ml
     here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "quantem-cuda_b200")
     if here not in sys.path:
         sys.path.insert(0, here)
     from quantem.cuda.core import ml
 
-    _ml = ml
     return ml
 
 
