@@ -341,15 +341,15 @@ PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
 }
 
 // (x, residual, weight, eps, out_dtype, look_for_grad) -> (y[, scale][, h]), the
-// scale for out_dtype e4m3; without a weight: x as it is in 8 bits; None as above
+// scale for out_dtype e4m3; None as above
 PyObject *norm(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     return guarded(n_args, 6, [&]() -> PyObject * {
         if (a[5] == Py_True && wants_grad(a, 3)) Py_RETURN_NONE;
-        const Arg x(a[0], false), r(a[1], true), w(a[2], true);
+        const Arg x(a[0], false), r(a[1], true), w(a[2], false);
         require(x.type != QC_E4M3 && x.dims >= 1 && x.last() > 0 && x.last() < (1 << 30));
         const long long n = x.last();
         const int out = type_of(a[4], x.type);
-        require(w.given() ? w.type == x.type && w.vector(n, x) : out == QC_E4M3 && !r.given());
+        require(w.type == x.type && w.vector(n, x));
         if (r.given()) require(r.type == x.type && r.alike(x));
         require(PyFloat_CheckExact(a[3]));
         require(out == x.type || out == QC_F32 || out == QC_E4M3 || x.type == QC_F32);
@@ -362,15 +362,28 @@ PyObject *norm(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
         const void *px = ptr<const void>(x.ptr);
         const long rows = (long)(x.count / n);
         float *ps = scale ? ptr<float>(address(scale)) : nullptr;
-        if (!w.given())
-            check(quantize_rows_cuda(px, ptr<void>(address(y)), ps, rows, (int)n, (long)n, x.type, stream));
-        else
-            check(rms_norm_cuda(px, ptr<const void>(r.ptr), ptr<const void>(w.ptr), ptr<void>(address(y)),
-                                h ? ptr<void>(address(h)) : nullptr, ps, rows, (int)n, (long)n, (long)n, x.type, out,
-                                (float)PyFloat_AS_DOUBLE(a[3]), stream));
+        check(rms_norm_cuda(px, ptr<const void>(r.ptr), ptr<const void>(w.ptr), ptr<void>(address(y)),
+                            h ? ptr<void>(address(h)) : nullptr, ps, rows, (int)n, (long)n, (long)n, x.type, out,
+                            (float)PyFloat_AS_DOUBLE(a[3]), stream));
         if (scale && h) return PyTuple_Pack(3, y.get(), scale.get(), h.get());
         if (scale || h) return PyTuple_Pack(2, y.get(), scale ? scale.get() : h.get());
         return PyTuple_Pack(1, y.get());
+    });
+}
+
+// (x, look_for_grad) -> (q, scale); None as above
+PyObject *quantize(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
+    return guarded(n_args, 2, [&]() -> PyObject * {
+        if (a[1] == Py_True && wants_grad(a, 1)) Py_RETURN_NONE;
+        const Arg x(a[0], false);
+        require(x.type != QC_E4M3 && x.dims >= 1 && x.last() > 0 && x.last() < (1 << 30));
+        const long long n = x.last();
+        const cudaStream_t stream = stream_on(x);
+        Ref q = new_tensor(x, shape_of(x, n).get(), dtypes[QC_E4M3]);
+        Ref scale = new_tensor(x, shape_of(x, -1).get(), x.type == QC_F32 ? nullptr : dtypes[QC_F32]);
+        check(quantize_rows_cuda(ptr<const void>(x.ptr), ptr<void>(address(q)), ptr<float>(address(scale)),
+                                 (long)(x.count / n), (int)n, (long)n, x.type, stream));
+        return PyTuple_Pack(2, q.get(), scale.get());
     });
 }
 
@@ -435,6 +448,8 @@ PyMethodDef methods[] = {
      "Backward of linear_act from the kept derivative, or NotImplemented."},
     {"decoder_norm", (PyCFunction)(void (*)(void))norm, METH_FASTCALL,
      "RMS norm for plain contiguous tensors, or NotImplemented."},
+    {"decoder_quantize", (PyCFunction)(void (*)(void))quantize, METH_FASTCALL,
+     "quantize_rows_fp8 for plain contiguous tensors, or NotImplemented."},
     {"decoder_norm_grad", (PyCFunction)(void (*)(void))norm_grad, METH_FASTCALL,
      "Backward of the RMS norm for plain contiguous tensors, or NotImplemented."},
     {nullptr, nullptr, 0, nullptr},

@@ -79,6 +79,12 @@ def _no_backward(fn: str, *tensors: Tensor | None) -> None:
         raise RuntimeError(f"{fn} has no backward: call it under torch.no_grad() or detach its inputs")
 
 
+def _given(fn: str, **tensors) -> None:
+    for name, x in tensors.items():
+        if not isinstance(x, Tensor):
+            raise TypeError(f"{fn}: {name} must be a tensor, got {type(x).__name__}")
+
+
 def _check(fn: str, name: str, x: Tensor, shape: tuple[int, ...], dtypes: tuple[torch.dtype, ...],
            device: torch.device) -> None:
     if x.dtype not in dtypes:
@@ -131,6 +137,7 @@ def _ptr(x: Tensor | None) -> int:
 
 
 def _check_norm(fn: str, x: Tensor, residual: Tensor | None, weight: Tensor) -> None:
+    _given(fn, x=x, weight=weight)
     _check_rows(fn, "x", x, _FLOATS)
     if residual is not None:
         _check(fn, "residual", residual, x.shape, (x.dtype,), x.device)
@@ -365,6 +372,7 @@ def _(x, residual, weight, eps):
 
 
 def _quantize_impl(x: Tensor) -> tuple[Tensor, Tensor]:
+    _given("quantize_rows_fp8", x=x)
     _check_rows("quantize_rows_fp8", "x", x, _FLOATS)
     x2, rows, stride = _rows(x)
     q = x.new_empty(x.shape, dtype=_FP8)
@@ -389,6 +397,7 @@ def _norm_fp8_call(fn: str, x: Tensor, residual: Tensor | None, weight: Tensor, 
         outs = _core.decoder_norm(x, residual, weight, eps, _FP8, True)
         if outs is not NotImplemented and outs is not None:
             return outs
+    _given(fn, x=x, weight=weight)
     _no_backward(fn, x, residual, weight)
     if not _plain(x, residual, weight):
         _check_norm(fn, x, residual, weight)
@@ -422,7 +431,7 @@ def quantize_rows_fp8(x: Tensor) -> tuple[Tensor, Tensor]:
     scale per row, ``x ≈ q * scale[..., None]``: the weights ``[N, K]`` and
     inputs of :func:`linear_act_fp8`. No backward."""
     if not _is_compiling():
-        outs = _core.decoder_norm(x, None, None, 0.0, _FP8, True)
+        outs = _core.decoder_quantize(x, True)
         if outs is not NotImplemented and outs is not None:
             return outs
     _no_backward("quantize_rows_fp8", x)
@@ -451,6 +460,7 @@ def _check_linear(fn: str, x: Tensor, weight: Tensor, bias: Tensor | None, resid
 
 
 def _check_linear16(fn: str, x, weight, bias, residual, activation, out_dtype) -> torch.dtype:
+    _given(fn, x=x, weight=weight)
     out = x.dtype if out_dtype is None else out_dtype
     _check_linear(fn, x, weight, bias, residual, activation, out, _HALVES, (x.dtype, torch.float32),
                   (x.dtype, torch.float32))
@@ -621,6 +631,7 @@ def linear_act(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual: 
 
 def _check_linear8(x, x_scale, weight, weight_scale, bias, residual, activation, out_dtype) -> None:
     fn = "linear_act_fp8"
+    _given(fn, x=x, x_scale=x_scale, weight=weight, weight_scale=weight_scale)
     _check_linear(fn, x, weight, bias, residual, activation, out_dtype, (_FP8,), _FLOATS, _FLOATS)
     _check(fn, "x_scale", x_scale, x.shape[:-1], (torch.float32,), x.device)
     _check(fn, "weight_scale", weight_scale, weight.shape[:1], (torch.float32,), x.device)
@@ -662,10 +673,11 @@ def linear_act_fp8(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Ten
 
     Accumulation and epilogue are fp32, rounded once. No backward.
     """
-    if not _is_compiling():
+    if x_scale is not None and not _is_compiling():  # without scales, the direct call takes 16-bit operands
         y = _core.decoder_linear(x, weight, bias, residual, x_scale, weight_scale, activation, out_dtype, True)
         if y is not NotImplemented and y is not None:
             return y
+    _given("linear_act_fp8", x=x, x_scale=x_scale, weight=weight, weight_scale=weight_scale)
     _no_backward("linear_act_fp8", bias, residual, x_scale, weight_scale)
     args = (x, x_scale, weight, weight_scale, bias, residual, activation, out_dtype)
     if _plain(x, x_scale, weight, weight_scale, bias, residual):
