@@ -14,13 +14,15 @@ bits (e4m3 with scales) for serving.
 The features come as fp32 ``[points, T*C]``; the norm's ``out_dtype`` takes
 them to the decoder's type. As in the K-Planes layer, the public wrappers call
 the implementations directly when they run eagerly, and the registered ops
-under ``torch.compile`` and for tensor subclasses.
+while a graph is recorded (``torch.compile``, ``make_fx``, ``torch.jit.trace``)
+and for tensor subclasses. Forward-mode derivatives are refused.
 """
 
 from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from quantem.cuda import _core
 
@@ -39,6 +41,26 @@ _FP8 = torch.float8_e4m3fn
 _core.decoder_setup(Tensor, torch.nn.Parameter, (torch.float32, torch.bfloat16, torch.float16, _FP8), torch.uint8,
                     torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled, _ACT)
 _is_compiling = torch.compiler.is_compiling
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_early_modes = torch._ops._len_torch_dispatch_stack_pre_dispatch
+_trace = torch._C._get_tracing_state
+
+
+def _direct() -> bool:
+    """Whether a call may pass torch's dispatcher by. Not while a graph is
+    recorded, which would hold the outputs' allocations alone; not inside a
+    forward-mode level, whose tangents those allocations would drop."""
+    return not (_is_compiling() or forward_ad._current_level >= 0 or _dispatch_modes() or _early_modes()
+                or _trace() is not None)
+
+
+def _no_forward_mode(fn: str, *tensors: Tensor | None) -> None:
+    """Refuses tangents (the registered ops would drop them)."""
+    if forward_ad._current_level < 0:
+        return
+    for x in tensors:
+        if isinstance(x, Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+            raise NotImplementedError(f"{fn} has no forward-mode derivative")
 
 
 def _launch(entry, x: Tensor, *args) -> None:
@@ -55,11 +77,11 @@ _PLAIN = {Tensor, torch.nn.Parameter, type(None)}
 
 
 def _plain(*tensors: Tensor | None) -> bool:
-    """True for plain tensors and parameters outside torch.compile."""
+    """True for plain tensors and parameters of a direct call."""
     for x in tensors:
         if type(x) not in _PLAIN:
             return False
-    return not _is_compiling()
+    return _direct()
 
 
 def _wants_grad(*tensors: Tensor | None) -> bool:
@@ -285,20 +307,25 @@ class _RmsNorm(torch.autograd.Function):
         if dy is None:  # only the sum h took part in the loss: its gradient passes through
             dw = torch.zeros(weight.shape, dtype=weight.dtype, device=weight.device) if need_w else None
             return None, dh if need_x else None, dh if need_r else None, dw, None, None
-        dx, dw = _rms_norm_bwd_impl(x, residual, weight, dy, dh, ctx.eps, need_x or need_r, need_w)
+        if _direct():
+            dx, dw = _rms_norm_bwd_impl(x, residual, weight, dy, dh, ctx.eps, need_x or need_r, need_w)
+        else:
+            _no_forward_mode("rms_norm_bwd", dy, dh)
+            dx, dw = _rms_norm_bwd(x, residual, weight, dy, dh, ctx.eps)
         return None, dx if need_x else None, dx if need_r else None, dw, None, None
 
 
 def _norm_call(fn: str, x: Tensor, residual: Tensor | None, weight: Tensor, eps: float,
                out_dtype: torch.dtype | None):
     eps = float(eps)
-    if out_dtype is not _FP8 and not _is_compiling():
+    if out_dtype is not _FP8 and _direct():
         outs = _core.decoder_norm(x, residual, weight, eps, out_dtype, True)
         if outs is None:  # plain tensors, a gradient is recorded
             return _RmsNorm.apply(fn, x, residual, weight, eps, out_dtype)
         if outs is not NotImplemented:
             return outs
     if not _plain(x, residual, weight):
+        _no_forward_mode(fn, x, residual, weight)
         _check_norm(fn, x, residual, weight)
         _norm_out_dtype(fn, x, out_dtype)
         return _rms_norm(x, residual, weight, eps, out_dtype)
@@ -393,13 +420,14 @@ def _(x):
 
 
 def _norm_fp8_call(fn: str, x: Tensor, residual: Tensor | None, weight: Tensor, eps: float):
-    if not _is_compiling():
+    if _direct():
         outs = _core.decoder_norm(x, residual, weight, eps, _FP8, True)
         if outs is not NotImplemented and outs is not None:
             return outs
     _given(fn, x=x, weight=weight)
     _no_backward(fn, x, residual, weight)
     if not _plain(x, residual, weight):
+        _no_forward_mode(fn, x, residual, weight)
         _check_norm(fn, x, residual, weight)
         return _rms_norm_fp8(x, residual, weight, eps)
     return _rms_norm_fp8_impl(fn, x, residual, weight, eps)
@@ -430,12 +458,15 @@ def quantize_rows_fp8(x: Tensor) -> tuple[Tensor, Tensor]:
     """Rows of ``x`` (fp32, bf16 or fp16 ``[..., n]``) as e4m3 with one fp32
     scale per row, ``x ≈ q * scale[..., None]``: the weights ``[N, K]`` and
     inputs of :func:`linear_act_fp8`. No backward."""
-    if not _is_compiling():
+    if _direct():
         outs = _core.decoder_quantize(x, True)
         if outs is not NotImplemented and outs is not None:
             return outs
     _no_backward("quantize_rows_fp8", x)
-    return _quantize_impl(x) if _plain(x) else _quantize_rows_fp8(x)
+    if _plain(x):
+        return _quantize_impl(x)
+    _no_forward_mode("quantize_rows_fp8", x)
+    return _quantize_rows_fp8(x)
 
 
 # ── matrix product with epilogue ──────────────────────────────────────────
@@ -550,7 +581,10 @@ def _linear_setup(ctx, inputs, output) -> None:
 
 
 def _linear_backward(ctx, dy):
-    x, weight, bias = ctx.saved_tensors
+    return _linear_backward_op(ctx, *ctx.saved_tensors, dy)
+
+
+def _linear_backward_op(ctx, x, weight, bias, dy):
     nx, nw, nb, nr = ctx.needs_input_grad[:4]
     need = [nx, nw, nb and bias is not None]
     got = iter(_linear_act_bwd(x, weight, bias, dy, ctx.activation, need) if any(need) else [])
@@ -581,6 +615,9 @@ class _LinearAct(torch.autograd.Function):
         x, weight, bias, kept = ctx.saved_tensors
         nx, nw, nb, nr = ctx.needs_input_grad[:4]
         dx = dw = db = None
+        if not _direct():
+            _no_forward_mode("linear_act_bwd", dy)
+            return _linear_backward_op(ctx, x, weight, bias, dy)
         if kept is not None and (nx or nw or nb):
             grads = _core.decoder_linear_grad_kept(x, weight, kept, dy, ctx.activation, nx, nw, nb)
             if grads is not NotImplemented:
@@ -615,13 +652,14 @@ def linear_act(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual: 
     Widths and addresses that no 16-byte boundary divides are handled by a copy
     of the operand to padded rows; multiples of 8 features avoid it.
     """
-    if not _is_compiling():
+    if _direct():
         y = _core.decoder_linear(x, weight, bias, residual, None, None, activation, out_dtype, True)
         if y is None:  # plain tensors, a gradient is recorded
             return _LinearAct.apply(x, weight, bias, residual, activation, out_dtype)
         if y is not NotImplemented:
             return y
     if not _plain(x, weight, bias, residual):
+        _no_forward_mode("linear_act", x, weight, bias, residual)
         _check_linear16("linear_act", x, weight, bias, residual, activation, out_dtype)
         return _linear_act(x, weight, bias, residual, activation, out_dtype)
     if _wants_grad(x, weight, bias, residual):
@@ -673,7 +711,7 @@ def linear_act_fp8(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Ten
 
     Accumulation and epilogue are fp32, rounded once. No backward.
     """
-    if x_scale is not None and not _is_compiling():  # without scales, the direct call takes 16-bit operands
+    if x_scale is not None and _direct():  # without scales, the direct call takes 16-bit operands
         y = _core.decoder_linear(x, weight, bias, residual, x_scale, weight_scale, activation, out_dtype, True)
         if y is not NotImplemented and y is not None:
             return y
@@ -682,5 +720,6 @@ def linear_act_fp8(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Ten
     args = (x, x_scale, weight, weight_scale, bias, residual, activation, out_dtype)
     if _plain(x, x_scale, weight, weight_scale, bias, residual):
         return _linear8_impl(*args)
+    _no_forward_mode("linear_act_fp8", x_scale, weight_scale, bias, residual)
     _check_linear8(*args)
     return _linear_act_fp8(*args)

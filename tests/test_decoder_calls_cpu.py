@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from quantem.cuda.core import ml
 
@@ -31,3 +32,25 @@ def _t(*shape, dtype=BF16):
 def test_missing_tensors_are_refused(call, match):
     with pytest.raises(TypeError, match=rf"\b{match}\b.*must be a tensor"):
         call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda x, d: ml.rms_norm(x, d(_t(8))),
+    lambda x, d: ml.rms_norm(d(x), _t(8)),
+    lambda x, d: ml.add_rms_norm(x, d(x), _t(8)),
+    lambda x, d: ml.rms_norm_fp8(d(x), _t(8)),
+    lambda x, d: ml.add_rms_norm_fp8(x, d(x), _t(8)),
+    lambda x, d: ml.quantize_rows_fp8(d(x)),
+    lambda x, d: ml.linear_act(d(x), _t(6, 8)),
+    lambda x, d: ml.linear_act(x, _t(6, 8), residual=d(_t(4, 6))),
+    lambda x, d: ml.linear_act_fp8(_t(4, 8, dtype=E4M3), d(_t(4, dtype=F32)), _t(6, 8, dtype=E4M3), _t(6, dtype=F32)),
+])
+def test_forward_mode_derivatives_are_refused(call):
+    x = _t(4, 8)
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(x, lambda t: fwd.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(ValueError, match="CUDA"):  # without tangents: the usual checks
+            call(x, lambda t: t)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: ml.rms_norm(t, _t(8)), (x,), (x,))
