@@ -58,7 +58,7 @@ struct Names {
 constexpr int kTypes = 4;
 // What setup() was given, kept for the life of the process.
 PyObject *tensor_type, *parameter_type, *dtypes[kTypes], *uint8_dtype, *current_device, *current_stream, *grad_enabled,
-    *activations;
+    *activations, *dispatch_modes, *function_modes, *forward_ad, *forward_ad_level;
 
 PyObject *checked(PyObject *p) {
     if (!p) throw Raised();
@@ -110,7 +110,9 @@ struct Arg {
         require(PyTuple_Check(s.get()) && PyTuple_GET_SIZE(s.get()) <= kMaxDims);
         dims = (int)PyTuple_GET_SIZE(s.get());
         for (int i = 0; i < dims; ++i) {
-            size[i] = as_int(PyTuple_GET_ITEM(s.get(), i));
+            PyObject *v = PyTuple_GET_ITEM(s.get(), i);
+            require(PyLong_CheckExact(v));  // torch.jit.trace gives tensors
+            size[i] = as_int(v);
             count *= size[i];
         }
         ptr = (uintptr_t)call_int(o, names.data_ptr);
@@ -132,6 +134,18 @@ struct Arg {
         return n < 0 || last() == n;
     }
 };
+
+// A call that comes straight from a user: none that a mode records (make_fx has
+// a function mode where it has no dispatch mode) and none inside a forward-mode
+// level, whose tangents the outputs' allocations would drop.
+void require_direct() {
+    Ref level(checked(PyObject_GetAttr(forward_ad, forward_ad_level)));
+    require(as_int(level.get()) < 0);
+    Ref d(checked(PyObject_CallNoArgs(dispatch_modes)));
+    require(as_int(d.get()) == 0);
+    Ref f(checked(PyObject_CallNoArgs(function_modes)));
+    require(as_int(f.get()) == 0);
+}
 
 // Whether a gradient is recorded for one of the plain tensors (or None) in
 // a[0..n); asked before anything else, as the answer sends the call on.
@@ -219,11 +233,14 @@ PyObject *guarded(Py_ssize_t got, Py_ssize_t want, F &&body) {
     }
 }
 
-// (x, weight, bias, residual, x_scale, weight_scale, activation, out_dtype, look_for_grad) -> y,
-// or None where the tensors are plain and a gradient is recorded
+// (x, weight, bias, residual, x_scale, weight_scale, activation, out_dtype, from_user) -> y,
+// or None where a user's tensors are plain and a gradient is recorded
 PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     return guarded(n_args, 9, [&]() -> PyObject * {
-        if (a[8] == Py_True && wants_grad(a, 6)) Py_RETURN_NONE;
+        if (a[8] == Py_True) {
+            require_direct();
+            if (wants_grad(a, 6)) Py_RETURN_NONE;
+        }
         const Arg x(a[0], false), w(a[1], false), b(a[2], true), r(a[3], true), sx(a[4], true), sw(a[5], true);
         const bool f8 = sx.given();
         require(x.type == w.type && (f8 ? x.type == QC_E4M3 : is_16bit(x.type)) && x.dims >= 1 && w.dims == 2);
@@ -340,11 +357,14 @@ PyObject *linear_grad(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     });
 }
 
-// (x, residual, weight, eps, out_dtype, look_for_grad) -> (y[, scale][, h]), the
+// (x, residual, weight, eps, out_dtype, from_user) -> (y[, scale][, h]), the
 // scale for out_dtype e4m3; None as above
 PyObject *norm(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     return guarded(n_args, 6, [&]() -> PyObject * {
-        if (a[5] == Py_True && wants_grad(a, 3)) Py_RETURN_NONE;
+        if (a[5] == Py_True) {
+            require_direct();
+            if (wants_grad(a, 3)) Py_RETURN_NONE;
+        }
         const Arg x(a[0], false), r(a[1], true), w(a[2], false);
         require(x.type != QC_E4M3 && x.dims >= 1 && x.last() > 0 && x.last() < (1 << 30));
         const long long n = x.last();
@@ -371,10 +391,13 @@ PyObject *norm(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     });
 }
 
-// (x, look_for_grad) -> (q, scale); None as above
+// (x, from_user) -> (q, scale); None as above
 PyObject *quantize(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     return guarded(n_args, 2, [&]() -> PyObject * {
-        if (a[1] == Py_True && wants_grad(a, 1)) Py_RETURN_NONE;
+        if (a[1] == Py_True) {
+            require_direct();
+            if (wants_grad(a, 1)) Py_RETURN_NONE;
+        }
         const Arg x(a[0], false);
         require(x.type != QC_E4M3 && x.dims >= 1 && x.last() > 0 && x.last() < (1 << 30));
         const long long n = x.last();
@@ -415,9 +438,10 @@ PyObject *norm_grad(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
 }
 
 // (Tensor, Parameter, (dtypes in the order of QC_F32..QC_E4M3), uint8, current
-// device's index, raw current stream, is_grad_enabled, {activation: code})
+// device's index, raw current stream, is_grad_enabled, {activation: code},
+// dispatch modes' and function modes' number, torch.autograd.forward_ad)
 PyObject *setup(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
-    return guarded(n_args, 8, [&]() -> PyObject * {
+    return guarded(n_args, 11, [&]() -> PyObject * {
         require(PyTuple_Check(a[2]) && PyTuple_GET_SIZE(a[2]) == kTypes && PyDict_Check(a[7]));
         const char *words[] = {"shape", "dtype", "data_ptr", "is_contiguous", "get_device", "new_empty", "requires_grad"};
         PyObject **to[] = {&names.shape,      &names.dtype,     &names.data_ptr,     &names.is_contiguous,
@@ -432,6 +456,10 @@ PyObject *setup(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
         current_stream = Py_NewRef(a[5]);
         grad_enabled = Py_NewRef(a[6]);
         activations = Py_NewRef(a[7]);
+        dispatch_modes = Py_NewRef(a[8]);
+        function_modes = Py_NewRef(a[9]);
+        forward_ad = Py_NewRef(a[10]);
+        forward_ad_level = checked(PyUnicode_InternFromString("_current_level"));
         Py_RETURN_NONE;
     });
 }

@@ -33,15 +33,17 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _HALVES = (torch.bfloat16, torch.float16)
 _FP8 = torch.float8_e4m3fn
 
-# The common calls (plain contiguous tensors on the current device) run in the
-# extension from their checks to the launch; they return NotImplemented for
-# anything else, which the functions below then check, convert or refuse.
-# (_cuda_getCurrentRawStream gives the stream's handle; torch.cuda.current_stream
-# builds a stream object first, 2 us of a 10 us call.)
-_core.decoder_setup(Tensor, torch.nn.Parameter, (torch.float32, torch.bfloat16, torch.float16, _FP8), torch.uint8,
-                    torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled, _ACT)
-_is_compiling = torch.compiler.is_compiling
 _dispatch_modes = torch._C._len_torch_dispatch_stack
+
+# The common calls (plain contiguous tensors on the current device, no modes)
+# run in the extension from their checks to the launch; they return
+# NotImplemented for anything else, which the functions below then check,
+# convert or refuse. (_cuda_getCurrentRawStream gives the stream's handle;
+# torch.cuda.current_stream builds a stream object first, 2 us of a 10 us call.)
+_core.decoder_setup(Tensor, torch.nn.Parameter, (torch.float32, torch.bfloat16, torch.float16, _FP8), torch.uint8,
+                    torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled, _ACT,
+                    _dispatch_modes, torch._C._len_torch_function_stack, forward_ad)
+_is_compiling = torch.compiler.is_compiling
 _early_modes = torch._ops._len_torch_dispatch_stack_pre_dispatch
 _trace = torch._C._get_tracing_state
 
@@ -318,11 +320,11 @@ class _RmsNorm(torch.autograd.Function):
 def _norm_call(fn: str, x: Tensor, residual: Tensor | None, weight: Tensor, eps: float,
                out_dtype: torch.dtype | None):
     eps = float(eps)
-    if out_dtype is not _FP8 and _direct():
+    if out_dtype is not _FP8 and not _is_compiling():
         outs = _core.decoder_norm(x, residual, weight, eps, out_dtype, True)
-        if outs is None:  # plain tensors, a gradient is recorded
+        if outs is None and _trace() is None:  # plain tensors, a gradient is recorded
             return _RmsNorm.apply(fn, x, residual, weight, eps, out_dtype)
-        if outs is not NotImplemented:
+        if outs is not NotImplemented and outs is not None:
             return outs
     if not _plain(x, residual, weight):
         _no_forward_mode(fn, x, residual, weight)
@@ -420,7 +422,7 @@ def _(x):
 
 
 def _norm_fp8_call(fn: str, x: Tensor, residual: Tensor | None, weight: Tensor, eps: float):
-    if _direct():
+    if not _is_compiling():
         outs = _core.decoder_norm(x, residual, weight, eps, _FP8, True)
         if outs is not NotImplemented and outs is not None:
             return outs
@@ -458,7 +460,7 @@ def quantize_rows_fp8(x: Tensor) -> tuple[Tensor, Tensor]:
     """Rows of ``x`` (fp32, bf16 or fp16 ``[..., n]``) as e4m3 with one fp32
     scale per row, ``x ≈ q * scale[..., None]``: the weights ``[N, K]`` and
     inputs of :func:`linear_act_fp8`. No backward."""
-    if _direct():
+    if not _is_compiling():
         outs = _core.decoder_quantize(x, True)
         if outs is not NotImplemented and outs is not None:
             return outs
@@ -652,11 +654,11 @@ def linear_act(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual: 
     Widths and addresses that no 16-byte boundary divides are handled by a copy
     of the operand to padded rows; multiples of 8 features avoid it.
     """
-    if _direct():
+    if not _is_compiling():
         y = _core.decoder_linear(x, weight, bias, residual, None, None, activation, out_dtype, True)
-        if y is None:  # plain tensors, a gradient is recorded
+        if y is None and _trace() is None:  # plain tensors, a gradient is recorded
             return _LinearAct.apply(x, weight, bias, residual, activation, out_dtype)
-        if y is not NotImplemented:
+        if y is not NotImplemented and y is not None:
             return y
     if not _plain(x, weight, bias, residual):
         _no_forward_mode("linear_act", x, weight, bias, residual)
@@ -711,7 +713,7 @@ def linear_act_fp8(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Ten
 
     Accumulation and epilogue are fp32, rounded once. No backward.
     """
-    if x_scale is not None and _direct():  # without scales, the direct call takes 16-bit operands
+    if x_scale is not None and not _is_compiling():  # without scales, the direct call takes 16-bit operands
         y = _core.decoder_linear(x, weight, bias, residual, x_scale, weight_scale, activation, out_dtype, True)
         if y is not NotImplemented and y is not None:
             return y
