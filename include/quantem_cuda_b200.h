@@ -495,8 +495,9 @@ int linear_act_cuda(const void *x, const void *weight, const void *bias, const v
 
 /* Backward of linear_act for 16-bit operands: dx[rows, k] and dweight[n, k] of
  * `type`, dbias[n] of bias_type, each written if not NULL (the residual's
- * gradient is dy). dy has `type` or QC_F32. Sums over rows are taken in a fixed
- * order. The workspace's size depends on the same arguments and on the device. */
+ * gradient is dy). dy has `type` or QC_F32; dz = dy activation'(z) is rounded to
+ * `type` for the products (QC_F16 from QC_F32: scaled by a power of two that brings
+ * the largest |dy| near fp16's). Sums over rows are taken in a fixed order. The workspace's size depends on the same arguments and on the device. */
 size_t linear_act_grad_workspace_bytes(const void *x, const void *weight, const void *dy, const void *dx,
                                        const void *dweight, const void *dbias, long rows, int n, int k, long x_stride,
                                        long weight_stride, long dy_stride, int type, int dy_type, int activation,

@@ -20,6 +20,13 @@
 //   16 bits would add as much as that. A pass over dy then gives dz (8192 rows
 //   of 1024 by 4096, SiLU: 44 us, against 80 us).
 //
+// fp16 has too few exponents for fp32 upstream gradients (a loss averaged over
+// many values, a scaled one): there dz is multiplied by a power of two S that
+// brings the largest |dy| to 2^14..2^15 (|act'| <= 1.13, so dz S stays below 2^16),
+// and dz W and dz^T x are multiplied by 1/S, which rounds nothing. dz then has
+// fp16's 11 bits next to the largest gradient, down to 2^-39 of it. The price
+// is a pass over dy for its maximum.
+//
 // Accumulation is fp32 in tensor memory; bias, activation, residual and scales
 // are applied to the fp32 value, which is rounded once.
 #include <algorithm>
@@ -220,8 +227,19 @@ struct Product {
     void *y;  // plain-store outputs: contiguous [M, N]
     uint4 *kept;  // act'(z) in fp16: [row tile][64-column slab][quarter][8 columns][32 rows]
     void *colsum;  // [row tiles][N]: fp32 partial sums, or the sums themselves where there is one row tile
+    // The largest finite |dy| as bits, or null: the act grad pass stores dz S,
+    // the products of dz S are divided by S.
+    const unsigned int *dy_max;
     int colsum_type, bias_type, out_type, act, res_mode, tma_store;
 };
+
+// The power of two that takes m (bits of a finite |value|) to [2^14, 2^15), as
+// far as it and its reciprocal are normal fp32 numbers; INV: its reciprocal.
+template <bool INV>
+__device__ __forceinline__ float gradient_scale(unsigned int m) {
+    const int e = min(14 + 127 - (int)(m >> 23), 126);
+    return __uint_as_float((unsigned int)(127 + (INV ? -e : e)) << 23);
+}
 
 constexpr int kGroups = 4;
 constexpr int kThreads = 64 + 128 * kGroups;
@@ -320,6 +338,13 @@ __device__ __forceinline__ void epilogue_32(const Product &p, float (&v)[32], un
                                             const float *bias, const float *col_scale, float row_scale,
                                             const float *dy_row, int dy_left, uint4 *kept) {
     const bool wide = EPI == kPartial || p.out_type == QC_F32;
+    if constexpr (EPI == kForward || EPI == kPartial) {
+        if (p.dy_max) {
+            const float s = gradient_scale<true>(*p.dy_max);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= s;
+        }
+    }
     if constexpr (EPI != kPartial) {
         if (p.row_scale) {
 #pragma unroll
@@ -383,6 +408,15 @@ __device__ __forceinline__ void epilogue_32(const Product &p, float (&v)[32], un
         for (int c = 0; c < 8; ++c)
             *reinterpret_cast<float4 *>(slab + slab_at(row, chunk0 + c)) =
                 make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    } else if (EPI == kActGrad && p.dy_max) {  // the column sums take v without S
+        const float s = gradient_scale<false>(*p.dy_max);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            float d[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = v[8 * c + i] * s;
+            *reinterpret_cast<uint4 *>(slab + slab_at(row, chunk0 + c)) = pack8(d, p.out_type);
+        }
     } else {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -1000,19 +1034,60 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const T *src, long long 
     }
 }
 
+// The largest finite |dy| as bits into *out (0 before): bits of non-negative
+// floats order like the floats, and a maximum does not depend on its order.
+__global__ void __launch_bounds__(256) largest_kernel(const float *dy, long long ld, long long rows, int n,
+                                                      unsigned int *out) {
+    __shared__ unsigned int sh[8];
+    const long long threads = (long long)gridDim.x * 256, id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int lane = threadIdx.x & 31;
+    unsigned int m = 0;
+    auto take = [&](float v) {
+        const unsigned int b = __float_as_uint(v) & 0x7fffffffu;
+        if (b < 0x7f800000u) m = max(m, b);
+    };
+    if (ld == n) {
+        const long long count = rows * n;
+        long long done = 0;
+        if ((reinterpret_cast<uintptr_t>(dy) & 15) == 0) {
+            const float4 *q = reinterpret_cast<const float4 *>(dy);
+#pragma unroll 4
+            for (long long i = id; i < count / 4; i += threads) {
+                const float4 v = q[i];
+                take(v.x), take(v.y), take(v.z), take(v.w);
+            }
+            done = count / 4 * 4;
+        }
+        for (long long i = done + id; i < count; i += threads) take(dy[i]);
+    } else {
+        for (long long r = id / 32; r < rows; r += threads / 32)
+            for (int c = lane; c < n; c += 32) take(dy[r * ld + c]);
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) sh[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = max(m, sh[i]);
+        if (m) atomicMax(out, m);
+    }
+}
+
 // dz = dy where there is no activation: cast to the operands' type (dst may be
-// null), and column sums of blocks of rows. 64 columns x 4 rows of threads.
+// null; times S where the largest |dy| is given), and column sums of blocks of rows. 64 columns x 4 rows of threads.
 __global__ void __launch_bounds__(256) cast_colsum_kernel(const void *dy, long long ld, int dy_type, void *dst,
                                                           long long ld_dst, int dst_type, void *colsum, int colsum_type,
-                                                          long long rows, int n, long long rows_per_block) {
+                                                          long long rows, int n, long long rows_per_block,
+                                                          const unsigned int *dy_max) {
     __shared__ float sh[4][64];
+    const float scale = dy_max ? gradient_scale<false>(*dy_max) : 1.f;
     const int c = blockIdx.x * 64 + (threadIdx.x & 63), ry = threadIdx.x >> 6;
     const long long r0 = blockIdx.y * rows_per_block, r1 = min(rows, r0 + rows_per_block);
     float s = 0.f;
     if (c < n)
         for (long long r = r0 + ry; r < r1; r += 4) {
             const float v = load_any(dy, r * ld + c, dy_type);
-            if (dst) store_any(dst, r * ld_dst + c, dst_type, v);
+            if (dst) store_any(dst, r * ld_dst + c, dst_type, v * scale);
             s += v;
         }
     if (!colsum) return;
@@ -1399,10 +1474,10 @@ int apply_packs(const Packs &k, Operand &x, Operand &w, long M, int N, int K, in
 
 struct GradPlan {
     Packs packs;
-    bool make_dz, vectors;
+    bool make_dz, vectors, scaled;
     long long ld_dz, ld_part, rows_per_block;
     int splits, sum_parts;
-    size_t at_dz, at_sum, at_part, bytes;
+    size_t at_dz, at_sum, at_part, at_max, bytes;
 };
 GradPlan plan_grad(const void *x, const void *w, const void *dy, long M, int N, int K, long ldx, long ldw, long lddy,
                    int type, int dy_type, int act, int want, int sms, bool kept = false) {
@@ -1414,6 +1489,8 @@ GradPlan plan_grad(const void *x, const void *w, const void *dy, long M, int N, 
     g.ld_dz = round_up(N, 8);
     const bool z_pass = act != QC_ACT_NONE && !kept;
     g.vectors = kept || (act == QC_ACT_NONE && tiled && N % 8 == 0);  // dz_kernel serves
+    g.scaled = type == QC_F16 && dy_type == QC_F32 && (want & 3);
+    if (g.scaled) g.at_max = c.take(sizeof(unsigned int));
     if (g.make_dz || z_pass) g.at_dz = c.take((size_t)M * g.ld_dz * 2);
     g.make_dz = g.make_dz || z_pass;
     if (want & 4) {
@@ -1645,6 +1722,14 @@ static int backward(const char *fn, const void *x, const void *weight, const voi
     void *sums = !(want & 4) ? nullptr : g.sum_parts == 1 ? dbias : ws + g.at_sum;
     const int sums_type = g.sum_parts == 1 ? bias_type : QC_F32;
     const CUtensorMap none = {};
+    unsigned int *dy_max = g.scaled ? reinterpret_cast<unsigned int *>(ws + g.at_max) : nullptr;
+    if (dy_max) {
+        QC_CUDA_TRY(cudaMemsetAsync(dy_max, 0, sizeof(*dy_max), stream), "cudaMemsetAsync");
+        const long long blocks = ((long long)rows * n + 4095) / 4096;
+        largest_kernel<<<(unsigned)std::min<long long>(blocks, (long long)sms * 8), 256, 0, stream>>>(
+            static_cast<const float *>(dy), dy_stride, rows, n, dy_max);
+        QC_CHECK_LAUNCH("largest_kernel");
+    }
 
     if (activation != QC_ACT_NONE && !kept) {
         Product p{};
@@ -1659,6 +1744,7 @@ static int backward(const char *fn, const void *x, const void *weight, const voi
         p.act = activation;
         p.colsum = sums;
         p.colsum_type = sums_type;
+        p.dy_max = dy_max;
         p.tma_store = 1;
         p.res_mode = dy_type == QC_F32 ? kResThread : tileable(dy, dy_stride, type) ? kResTma : kResWarp;
         CUtensorMap map_y = {}, map_r = {};
@@ -1684,7 +1770,7 @@ static int backward(const char *fn, const void *x, const void *weight, const voi
     } else if (g.make_dz || sums) {
         void *dst = g.make_dz ? ws + g.at_dz : nullptr;
         cast_colsum_kernel<<<dim3((n + 63) / 64, g.sum_parts), 256, 0, stream>>>(
-            dy, dy_stride, dy_type, dst, g.ld_dz, type, sums, sums_type, rows, n, g.rows_per_block);
+            dy, dy_stride, dy_type, dst, g.ld_dz, type, sums, sums_type, rows, n, g.rows_per_block, dy_max);
         QC_CHECK_LAUNCH("cast_colsum_kernel");
         if (g.make_dz) dzo = {ws + g.at_dz, g.ld_dz};
     }
@@ -1697,6 +1783,7 @@ static int backward(const char *fn, const void *x, const void *weight, const voi
         p.splits = 1;
         p.y = dx;
         p.out_type = type;
+        p.dy_max = dy_max;
         p.tma_store = tileable(dx, k, type);
         CUtensorMap map_y = {};
         if (p.tma_store)
@@ -1709,6 +1796,7 @@ static int backward(const char *fn, const void *x, const void *weight, const voi
         p.M = n;
         p.N = k;
         p.splits = g.splits;
+        p.dy_max = dy_max;
         CUtensorMap map_y = {};
         if (g.splits > 1) {
             float *part = reinterpret_cast<float *>(ws + g.at_part);

@@ -637,7 +637,10 @@ def linear_act(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual: 
 
     Differentiable w.r.t. ``x``, ``weight``, ``bias`` and ``residual``. The
     backward forms the activation's argument again; large bf16 calls keep its
-    derivative instead (2 bytes per output until the backward). Products
+    derivative instead (2 bytes per output until the backward). It rounds
+    dz = dy activation'(z) to x's type before the products with weight and x; fp32
+    gradients of fp16 calls are scaled by a power of two for it (dz below 2**-39
+    of the largest dy is lost), fp16 ones beyond 57000 may overflow. Products
     run on the tensor cores with fp32 accumulation, the epilogue is fp32, and
     ``y`` is rounded once. Sums over rows are taken in a fixed order: outputs
     and gradients are the same from run to run.
