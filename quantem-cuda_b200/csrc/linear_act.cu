@@ -16,9 +16,10 @@
 // * z is formed again from x and W, and the epilogue multiplies dy by act'(z):
 //   nothing is kept, nothing rounded but dz;
 // * a large bf16 forward keeps act'(z) itself, which lies within [-0.13, 1.13],
-//   in fp16: 2^-12 of its value off, an eighth of dz's own rounding, where z in
-//   16 bits would add as much as that. A pass over dy then gives dz (8192 rows
-//   of 1024 by 4096, SiLU: 44 us, against 80 us).
+//   in fp16 times 2^12: at most half a step off, 2^-11 of its value (an eighth of
+//   dz's own rounding) down to 2^-26, and 2^-37 below; z in 16 bits would add as
+//   much as dz's rounding. A pass over dy then gives dz (8192 rows of 1024 by
+//   4096, SiLU: 44 us, against 80 us).
 //
 // fp16 has too few exponents for fp32 upstream gradients (a loss averaged over
 // many values, a scaled one): there dz is multiplied by a power of two S that
@@ -46,6 +47,7 @@ namespace {
 
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s per barrier wait
 constexpr int kMaxDevices = 64;
+constexpr float kKeptScale = 4096.f;  // of the kept derivative in fp16
 
 // ── activations ──────────────────────────────────────────────────────────
 
@@ -225,7 +227,7 @@ struct Product {
     const void *res;  // residual (forward) or dy (act grad)
     long long ld_res;
     void *y;  // plain-store outputs: contiguous [M, N]
-    uint4 *kept;  // act'(z) in fp16: [row tile][64-column slab][quarter][8 columns][32 rows]
+    uint4 *kept;  // act'(z) kKeptScale in fp16: [row tile][64-column slab][quarter][8 columns][32 rows]
     void *colsum;  // [row tiles][N]: fp32 partial sums, or the sums themselves where there is one row tile
     // The largest finite |dy| as bits, or null: the act grad pass stores dz S,
     // the products of dz S are divided by S.
@@ -361,6 +363,8 @@ __device__ __forceinline__ void epilogue_32(const Product &p, float (&v)[32], un
             float d[8];
 #pragma unroll
             for (int i = 0; i < 8; i += 2) act_both<ACT>(v[8 * c + i], v[8 * c + i + 1], d[i], d[i + 1]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] *= kKeptScale;
             if (kept) kept[32 * c] = pack8(d, QC_F16);
         }
     }
@@ -1118,7 +1122,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const unsigned short *dy, long 
                 unpack8(kept[((((r >> 7) * gridDim.x + blockIdx.x) * 4 + ((r >> 5) & 3)) * 8 + chunk) * 32 + (r & 31)],
                         QC_F16, d);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= d[i];
+                for (int i = 0; i < 8; ++i) v[i] *= d[i] * (1.f / kKeptScale);
                 *reinterpret_cast<uint4 *>(dz + r * ld_dz + c) = pack8(v, type);
             }
 #pragma unroll

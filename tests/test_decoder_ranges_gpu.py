@@ -81,6 +81,15 @@ def test_kept_derivative_over_the_whole_range(act):
     _within(db, want, (want.abs() * 2.0**-11 + 2.0**-25 + 2.0**-19) * 1.01 + _half_step(want, BF16) * (1 + 2.0**-8), act)
 
 
+def test_small_kept_derivatives_keep_their_digits():
+    """SiLU's derivative down to -30 is between 1e-12 and 1e-4: bf16 holds it,
+    so the kept one has to, within a bf16 step (its evaluation, 2**-14 of the
+    value, its own rounding, 2**-11, or 2**-37, and bf16's half step)."""
+    db, z = _kept_derivative(torch.linspace(-30, -12, 1600).cuda(), "silu")
+    want = _act_grad(z, "silu")
+    _within(db, want, want.abs() * (2.0**-14 + 2.0**-11 + 2.0**-8) + 2.0**-37)
+
+
 # ── fp32 upstream gradients of fp16 operands ──────────────────────────────
 
 
