@@ -350,7 +350,7 @@ __device__ __forceinline__ void epilogue_32(const Product &p, float (&v)[32], un
     if constexpr (EPI != kPartial) {
         if (p.row_scale) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= row_scale * col_scale[i];
+            for (int i = 0; i < 32; ++i) v[i] = v[i] * row_scale * col_scale[i];  // the scales' product may leave fp32
         }
         if (p.bias) {
 #pragma unroll
@@ -815,7 +815,7 @@ struct FewEpilogue {
 #pragma unroll
             for (int i = 0; i < 8; ++i) rs[i] = c + i < end ? p.row_scale[r0 + c + i] : 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] *= rs[i] * col_scale;
+            for (int i = 0; i < 8; ++i) z[i] = z[i] * rs[i] * col_scale;
         }
         if (p.res) {
             const E *from = static_cast<const E *>(p.res) + (r0 + c) * p.ld_res + f;

@@ -1,5 +1,6 @@
 """The decoder operators where values leave the usual range: saturated
-activations with the kept derivative, upstream gradients beyond fp16's range.
+activations with the kept derivative, upstream gradients beyond fp16's range,
+scales whose product leaves fp32's.
 
 Tolerances are bounds, derived here before the first run, on top of those of a
 rounding (half a step of the type) and of a sum (2**-23 per term and addition).
@@ -166,3 +167,21 @@ def test_not_finite_gradients_stay_in_their_rows(act):
     assert not dx[~keep].isfinite().any()
     zero, = torch.autograd.grad(ml.linear_act(x, w, activation=act, out_dtype=F32), [x], torch.zeros_like(dy))
     assert not zero.any()
+
+
+# ── scales of 8-bit operands ──────────────────────────────────────────────
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_scales_whose_product_leaves_fp32(rows):
+    """The product is multiplied by one scale after the other, so neither a
+    product of scales below fp32's normal range nor one above it counts."""
+    k, n = 64, 40
+    x, w = torch.full((rows, k), 448.0, device="cuda").to(E4M3), torch.full((n, k), 448.0, device="cuda").to(E4M3)
+    sx, sw = torch.full((rows,), 3e-30, device="cuda"), torch.full((n,), 7e-13, device="cuda")
+    y = ml.linear_act_fp8(x, sx, w, sw, out_dtype=F32)
+    want = 448.0**2 * k * sx.to(D)[:, None] * sw.to(D)
+    _within(y, want, want * 2.0**-20)
+    zero = torch.zeros(rows, k, device="cuda").to(E4M3)
+    y = ml.linear_act_fp8(zero, torch.full_like(sx, 1e25), w, torch.full_like(sw, 1e20), out_dtype=F32)
+    assert not y.any()
