@@ -493,11 +493,23 @@ int linear_act_cuda(const void *x, const void *weight, const void *bias, const v
                     long weight_stride, long residual_stride, int type, int out_type, int bias_type, int activation,
                     void *workspace, size_t workspace_bytes, cudaStream_t stream);
 
+/* The form in which a product of linear_act runs on a device of `sms` SMs (0: the
+ * current one): form[0] 0 few rows (weights on the rows' side), 1 a tile per CTA, 2
+ * a tile per pair of CTAs; form[1] columns of a tile (few rows: rows of x); form[2]
+ * parts of the reduction; form[3] rounds of tiles. For reading profiles, and for
+ * tests that have to reach a form. */
+#define QC_PRODUCT_FORWARD 0
+#define QC_PRODUCT_DERIVATIVE 1 /* x weight^T again, with dy activation'(z) in its epilogue */
+#define QC_PRODUCT_DX 2
+#define QC_PRODUCT_DWEIGHT 3
+int linear_act_form(int product, long rows, int n, int k, int type, int sms, int *form);
+
 /* Backward of linear_act for 16-bit operands: dx[rows, k] and dweight[n, k] of
  * `type`, dbias[n] of bias_type, each written if not NULL (the residual's
  * gradient is dy). dy has `type` or QC_F32; dz = dy activation'(z) is rounded to
  * `type` for the products (QC_F16 from QC_F32: scaled by a power of two that brings
- * the largest |dy| near fp16's). Sums over rows are taken in a fixed order. The workspace's size depends on the same arguments and on the device. */
+ * the largest |dy| near fp16's). Sums over rows are taken in a fixed order. The
+ * workspace's size depends on the same arguments and on the device. */
 size_t linear_act_grad_workspace_bytes(const void *x, const void *weight, const void *dy, const void *dx,
                                        const void *dweight, const void *dbias, long rows, int n, int k, long x_stride,
                                        long weight_stride, long dy_stride, int type, int dy_type, int activation,

@@ -1304,49 +1304,67 @@ int launch_product(const Operand &a, const Operand &b, int type, long long K, co
 // Tile width and whether two CTAs share a tile: the least rounds of tiles over
 // the SMs times a round's cost. A round costs little more for a wider tile (a
 // reduction of 4096 in bf16, one round: 24.5 us for 64 columns, 24.9 for 128,
-// 32 for 256, in pairs 26 and 29), because the latency of its loads counts
+// 32 for 256, 29 for 256 in pairs), because the latency of its loads counts
 // more than their bytes; 2048 rows of 4096 by 1024 take 45 us in two rounds of
 // 64 columns and 27 us in one of 128. Pairs need two row tiles and a reduction
 // of at least 16 ring stages (1024 16-bit values): over 4096 they take 195
 // against 222 us (8192 rows, 4096 columns), over 1024 57 against 61 us, and
 // over 256, where memory and the epilogue bound the product, 71 against 65 us.
+// Pairs of 128 columns cost more than single CTAs (26 us) and never less rounds.
 constexpr int kPairStages = 16;
 struct TileChoice {
     int bn;
     bool pair;
+    long long rounds;
 };
 TileChoice choose_tile(long long M, int n, int k_blocks, int splits, int sms) {
     struct Option {
         int bn, pair, cost;
     };
-    constexpr Option options[] = {{256, 1, 120}, {256, 0, 135}, {128, 0, 107}, {128, 1, 112}, {64, 0, 100}};
-    TileChoice best{64, false};
+    constexpr Option options[] = {{256, 1, 120}, {256, 0, 135}, {128, 0, 107}, {64, 0, 100}};
+    TileChoice best{64, false, 0};
     long long least = -1;
     for (const Option &o : options) {
         if ((o.bn > 64 && n <= o.bn / 2) || (o.pair && (M <= 128 || k_blocks / splits < kPairStages))) continue;
         const long long rows = o.pair ? 256 : 128, slots = o.pair ? sms / 2 : sms;
         const long long tiles = (M + rows - 1) / rows * ((n + o.bn - 1) / o.bn) * splits;
-        const long long cost = (tiles + slots - 1) / slots * o.cost;
-        if (least < 0 || cost < least) least = cost, best = {o.bn, o.pair != 0};
+        const long long rounds = (tiles + slots - 1) / slots, cost = rounds * o.cost;
+        if (least < 0 || cost < least) least = cost, best = {o.bn, o.pair != 0, rounds};
     }
     return best;
 }
 
+// Ring stages of a reduction over K values.
+int stages_of(long long K, int type) { return (int)((K * elem_size(type) + 127) / 128); }
+
 template <bool F8, bool A_MN, bool B_MN, int EPI>
 int run_product(const Operand &a, const Operand &b, int type, long long K, const CUtensorMap &map_y,
                 const CUtensorMap &map_r, Product p, int sms, int dev, cudaStream_t stream) {
-    p.k_blocks = (int)((K + (F8 ? 127 : 63)) / (F8 ? 128 : 64));
+    p.k_blocks = stages_of(K, type);
     const TileChoice c = choose_tile(p.M, p.N, p.k_blocks, p.splits, sms);
 #define QC_RUN(BN, PAIR) \
     return launch_product<F8, A_MN, B_MN, BN, EPI, PAIR>(a, b, type, K, map_y, map_r, p, sms, dev, stream)
-    if (c.pair) {
-        if (c.bn == 256) QC_RUN(256, true);
-        QC_RUN(128, true);
-    }
+    if (c.pair) QC_RUN(256, true);
     if (c.bn == 256) QC_RUN(256, false);
     if (c.bn == 128) QC_RUN(128, false);
     QC_RUN(64, false);
 #undef QC_RUN
+}
+
+// Rows of x in a tile of the few-row form, and the parts of its reduction: as
+// many as fill the SMs, two ring stages each at least, from 8 stages on (4
+// stages in 2 parts: 10.6 against 6.3 us at 128 rows). Clusters of 8 fill at
+// most 3/4 of the SMs: two do not fit into every group of SMs that shares a
+// cluster's network, and a cluster left over runs after the others (16 of them
+// 19.6 us, 32 of 4 CTAs 13.9 us).
+int few_rows_tile(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+int few_rows_parts(long long rows, int n, int k_blocks, int sms) {
+    const long long tiles = (long long)((n + 127) / 128) * ((rows + few_rows_tile(rows) - 1) / few_rows_tile(rows));
+    int parts = 1;
+    while (parts < 8 && k_blocks >= 8 && 4 * parts <= k_blocks &&
+           2 * parts * tiles <= (parts == 4 ? sms * 3 / 4 : sms))
+        parts *= 2;
+    return parts;
 }
 
 template <bool F8, int BN>
@@ -1355,19 +1373,10 @@ int launch_few(const Operand &x, const Operand &w, int type, long long K, Produc
     CUtensorMap map_w, map_x;
     if (int st = make_map(&map_w, w.p, type, K, p.N, w.ld, 128, 2)) return st;
     if (int st = make_map(&map_x, x.p, type, K, p.M, x.ld, BN, 2)) return st;
-    p.k_blocks = (int)((K + (F8 ? 127 : 63)) / (F8 ? 128 : 64));
+    p.k_blocks = stages_of(K, type);
     p.idesc = tc::instr_desc(type == QC_BF16 ? 1 : 0, false, false, BN);
-    const int tiles = (p.N + 127) / 128;
+    const int tiles = (p.N + 127) / 128, parts = few_rows_parts(p.M, p.N, p.k_blocks, sms);
     const long long row_tiles = (p.M + BN - 1) / BN;
-    // As many parts of the reduction as fill the SMs, two ring stages each at
-    // least, from 8 stages on (4 stages in 2 parts: 10.6 against 6.3 us at 128
-    // rows). Clusters of 8 fill at most 3/4 of the SMs: two do not fit into
-    // every group of SMs that shares a cluster's network, and a cluster left
-    // over runs after the others (16 of them 19.6 us, 32 of 4 CTAs 13.9 us).
-    int parts = 1;
-    while (parts < 8 && p.k_blocks >= 8 && 4 * parts <= p.k_blocks &&
-           2 * parts * tiles * row_tiles <= (parts == 4 ? sms * 3 / 4 : sms))
-        parts *= 2;
     p.splits = parts;
     auto kernel = few_rows_kernel<F8, BN>;
     const size_t smem = sizeof(FewSmem<BN>) + 1024;
@@ -1399,7 +1408,7 @@ int launch_few(const Operand &x, const Operand &w, int type, long long K, Produc
 // rows: 12.1 against 15.1), from 64 stages with up to 128 (4096 by 1024, 1024
 // rows: 20.4 against 24.7 us; 4096 by 4096, 512 rows: equal).
 bool few_rows(long long rows, int n, int k, int type) {
-    const long long stages = ((long long)k * elem_size(type) + 127) / 128;
+    const long long stages = stages_of(k, type);
     const long long tiles = (rows + 127) / 128 * ((n + 127) / 128);
     return rows <= 64 || (stages >= 32 && tiles <= 32) || (stages >= 64 && tiles <= 128);
 }
@@ -1476,6 +1485,15 @@ int apply_packs(const Packs &k, Operand &x, Operand &w, long M, int N, int K, in
     return 0;
 }
 
+// Parts of dweight's reduction, which runs over the rows: split until the SMs are
+// filled, at least 512 rows (8 ring stages) each, and at most 32768, because the
+// tensor cores cut each addition (2^-24 of the sum a step: 2048 steps stay below
+// half a step of fp16).
+int weight_splits(long long rows, int n, int k, int sms) {
+    const long long tiles = (long long)((n + 127) / 128) * ((k + 255) / 256);
+    return (int)std::max<long long>({1, std::min<long long>(sms / tiles, rows / 512), (rows + 32767) / 32768});
+}
+
 struct GradPlan {
     Packs packs;
     bool make_dz, vectors, scaled;
@@ -1513,12 +1531,7 @@ GradPlan plan_grad(const void *x, const void *w, const void *dy, long M, int N, 
     }
     g.splits = 1;
     if (want & 2) {
-        // the reduction runs over the rows: split until the SMs are filled, at
-        // least 512 rows (8 ring stages) each, and at most 32768, because the
-        // tensor cores cut each addition (2^-24 of the sum a step: 2048 steps
-        // stay below half a step of fp16)
-        const long long tiles = (long long)((N + 127) / 128) * ((K + 255) / 256);
-        g.splits = (int)std::max<long long>({1, std::min<long long>(sms / tiles, M / 512), (M + 32767) / 32768});
+        g.splits = weight_splits(M, N, K, sms);
         g.ld_part = round_up(K, 4);
         if (g.splits > 1) g.at_part = c.take((size_t)g.splits * N * g.ld_part * 4);
     }
@@ -1546,6 +1559,37 @@ int ml_fault_word(unsigned int *word, int clear) {
 using namespace qc::ml;
 
 extern "C" {
+
+int linear_act_form(int product, long rows, int n, int k, int type, int sms, int *form) {
+    if (int st = check_shape("linear_act_form", rows, n, k, k, k, type)) return st;
+    QC_RETURN_IF(product < QC_PRODUCT_FORWARD || product > QC_PRODUCT_DWEIGHT || rows == 0 || !form,
+                 QC_ERR_INVALID_ARGUMENT, "linear_act_form: product %d, %ld rows", product, rows);
+    if (sms <= 0)
+        if (int st = qc::device_sm_count(&sms)) return st;
+    const int stages = stages_of(k, type);
+    TileChoice c{};
+    int parts = 1;
+    if (product == QC_PRODUCT_FORWARD && few_rows(rows, n, k, type)) {
+        form[0] = 0;
+        form[1] = few_rows_tile(rows);
+        form[2] = few_rows_parts(rows, n, stages, sms);
+        form[3] = 1;
+        return 0;
+    }
+    if (product == QC_PRODUCT_FORWARD || product == QC_PRODUCT_DERIVATIVE) {
+        c = choose_tile(rows, n, stages, 1, sms);
+    } else if (product == QC_PRODUCT_DX) {
+        c = choose_tile(rows, k, stages_of(n, type), 1, sms);
+    } else {
+        parts = weight_splits(rows, n, k, sms);
+        c = choose_tile(n, k, stages_of(rows, type), parts, sms);
+    }
+    form[0] = c.pair ? 2 : 1;
+    form[1] = c.bn;
+    form[2] = parts;
+    form[3] = (int)c.rounds;
+    return 0;
+}
 
 size_t linear_act_workspace_bytes(const void *x, const void *weight, long rows, int n, int k, long x_stride,
                                   long weight_stride, int type) {
@@ -1601,13 +1645,14 @@ static int forward(const char *fn, const void *x, const void *weight, const void
     p.act = activation;
     const bool f8 = type == QC_E4M3;
     if (!kept && few_rows(rows, n, k, type)) {
-        if (rows <= 16)
+        const int bn = few_rows_tile(rows);
+        if (bn == 16)
             return f8 ? launch_few<true, 16>(xo, wo, type, k, p, sms, dev, stream)
                       : launch_few<false, 16>(xo, wo, type, k, p, sms, dev, stream);
-        if (rows <= 32)
+        if (bn == 32)
             return f8 ? launch_few<true, 32>(xo, wo, type, k, p, sms, dev, stream)
                       : launch_few<false, 32>(xo, wo, type, k, p, sms, dev, stream);
-        if (rows <= 64)
+        if (bn == 64)
             return f8 ? launch_few<true, 64>(xo, wo, type, k, p, sms, dev, stream)
                       : launch_few<false, 64>(xo, wo, type, k, p, sms, dev, stream);
         return f8 ? launch_few<true, 128>(xo, wo, type, k, p, sms, dev, stream)

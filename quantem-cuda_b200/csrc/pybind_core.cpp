@@ -620,6 +620,17 @@ PYBIND11_MODULE(_core, m) {
         py::arg("bias_type"), py::arg("activation"), py::arg("ws_ptr"), py::arg("ws_bytes"), py::arg("stream_ptr"));
 
     m.def(
+        "linear_act_form",
+        [](int product, long rows, int n, int k, int type, int sms) {
+            int form[4];
+            check(linear_act_form(product, rows, n, k, type, sms, form));
+            return py::make_tuple(form[0], form[1], form[2], form[3]);
+        },
+        "(form, columns, parts, rounds) of a product: form 0 few rows, 1 single CTAs, 2 pairs; product 0 forward, "
+        "1 derivative pass, 2 dx, 3 dweight.",
+        py::arg("product"), py::arg("rows"), py::arg("n"), py::arg("k"), py::arg("type"), py::arg("sms") = 0);
+
+    m.def(
         "linear_act_grad_workspace_bytes",
         [](uintptr_t x, uintptr_t weight, uintptr_t dy, uintptr_t dx, uintptr_t dweight, uintptr_t dbias, long rows,
            int n, int k, long x_stride, long weight_stride, long dy_stride, int type, int dy_type, int activation,
