@@ -49,6 +49,14 @@ constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s per barrier wait
 constexpr int kMaxDevices = 64;
 constexpr float kKeptScale = 4096.f;  // of the kept derivative in fp16
 
+// Value i of an array of `total` (debug build; always true otherwise). What TMA
+// moves is bounded by its tensor map.
+__device__ __forceinline__ bool in_array(long long i, long long total) {
+    return QC_IN_BOUNDS(i, total, g_ml_fault_word);
+}
+// Values of `rows` rows of n values, ld apart.
+__device__ __forceinline__ long long extent(long long rows, long long ld, int n) { return (rows - 1) * ld + n; }
+
 // ── activations ──────────────────────────────────────────────────────────
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -235,6 +243,11 @@ struct Product {
     int colsum_type, bias_type, out_type, act, res_mode, tma_store;
 };
 
+// 8-column vectors of the kept derivative: 1024 per 128 rows and 64 columns
+__host__ __device__ __forceinline__ long long kept_vectors(long long rows, int n) {
+    return (rows + 127) / 128 * ((n + 63) / 64) * 1024;
+}
+
 // The power of two that takes m (bits of a finite |value|) to [2^14, 2^15), as
 // far as it and its reciprocal are normal fp32 numbers; INV: its reciprocal.
 template <bool INV>
@@ -365,7 +378,7 @@ __device__ __forceinline__ void epilogue_32(const Product &p, float (&v)[32], un
             for (int i = 0; i < 8; i += 2) act_both<ACT>(v[8 * c + i], v[8 * c + i + 1], d[i], d[i + 1]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) d[i] *= kKeptScale;
-            if (kept) kept[32 * c] = pack8(d, QC_F16);
+            if (kept && in_array(kept + 32 * c - p.kept, kept_vectors(p.M, p.N))) kept[32 * c] = pack8(d, QC_F16);
         }
     }
     if constexpr (is_forward(EPI)) {
@@ -396,7 +409,10 @@ __device__ __forceinline__ void epilogue_32(const Product &p, float (&v)[32], un
         for (int i = 0; i < 32; i += 2) act_grad<ACT>(v[i], v[i + 1]);
         if (p.res_mode == kResThread) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = i < dy_left ? v[i] * dy_row[i] : 0.f;
+            for (int i = 0; i < 32; ++i)
+                v[i] = i < dy_left && in_array(dy_row + i - static_cast<const float *>(p.res), extent(p.M, p.ld_res, p.N))
+                           ? v[i] * dy_row[i]
+                           : 0.f;
         } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -449,12 +465,13 @@ __device__ __forceinline__ void slab_warp_copy(const Product &p, unsigned char *
                                                long long m0, int row0, int col0, int lane) {
     const bool wide = p.out_type == QC_F32;
     const int rows = (int)min(32ll, p.M - (m0 + row0)), cols = min(wide ? 32 : 64, p.N - col0);
+    const long long room = extent(p.M, ld, p.N);
 #pragma unroll 4
     for (int r = 0; r < rows; ++r) {
         const int row = row0 + r;
         const long long at = (m0 + row) * ld + col0;
         if (wide) {
-            if (lane < cols) {
+            if (lane < cols && in_array(at + lane, room)) {
                 float *s = reinterpret_cast<float *>(slab + slab_at(row, lane >> 2)) + (lane & 3);
                 float *g = static_cast<float *>(global) + at + lane;
                 if constexpr (LOAD) *s = *g;
@@ -464,7 +481,7 @@ __device__ __forceinline__ void slab_warp_copy(const Product &p, unsigned char *
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int c = lane + 32 * h;
-                if (c < cols) {
+                if (c < cols && in_array(at + c, room)) {
                     unsigned short *s = reinterpret_cast<unsigned short *>(slab + slab_at(row, c >> 3)) + (c & 7);
                     unsigned short *g = static_cast<unsigned short *>(global) + at + c;
                     if constexpr (LOAD) *s = *g;
@@ -640,11 +657,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const long long r = (long long)m * 128 + row;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const bool in = c + 32 * h < p.N;
+                const bool in = c + 32 * h < p.N && in_array(c + 32 * h, p.N);
                 if (p.bias) ahead.bias[h] = in ? load_any(p.bias, c + 32 * h, p.bias_type) : 0.f;
                 if (p.row_scale) ahead.scale[h] = in ? p.col_scale[c + 32 * h] : 0.f;
             }
-            if (p.row_scale) ahead.row_scale = r < p.M ? p.row_scale[r] : 0.f;
+            if (p.row_scale) ahead.row_scale = r < p.M && in_array(r, p.M) ? p.row_scale[r] : 0.f;
         };
         if constexpr (EPI != kPartial) look_ahead(0);
 
@@ -746,7 +763,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if constexpr (EPI == kActGrad) {
                     const int c = (ew & 3) * 32 + lane;
-                    if (p.colsum && c < 64 && col0 + c < p.N && m0 < p.M) {
+                    if (p.colsum && c < 64 && col0 + c < p.N && m0 < p.M &&
+                        in_array((long long)m * p.N + col0 + c, (p.M + 127) / 128 * p.N)) {
                         const float *cs = &sm.colsum[group][j & 1][0][c];
                         store_any(p.colsum, (long long)m * p.N + col0 + c, p.colsum_type,
                                   (cs[0] + cs[64]) + (cs[128] + cs[192]));
@@ -806,7 +824,7 @@ struct FewEpilogue {
 
     // sums z of rows c..c+8 of this tile, as far as `end`
     __device__ __forceinline__ void finish(float (&z)[8], int c, int end) const {
-        if (f >= p.N) return;
+        if (f >= p.N || !in_array(f, p.N) || !in_array(r0 + min(c + 8, end) - 1, p.M)) return;
         using E = typename ElemOf<OT>::type;
         const long long at = (r0 + c) * p.N + f;
         float res[8] = {};
@@ -1015,6 +1033,8 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const T *src, long long 
         const long long r = i / vecs;
         const int c = (int)(i - r * vecs) * V;
         const T *from = src + r * ld_src + c;
+        if (!in_array(r * ld_src + min(c + V, n) - 1, extent(rows, ld_src, n)) || !in_array(r * ld_dst + c + V - 1, rows * ld_dst))
+            continue;
         uint32_t w[4] = {0, 0, 0, 0};
         if (sizeof(T) == 2 && c + V <= n) {
             if ((reinterpret_cast<uintptr_t>(from) & 3) == 0) {
@@ -1057,6 +1077,7 @@ __global__ void __launch_bounds__(256) largest_kernel(const float *dy, long long
             const float4 *q = reinterpret_cast<const float4 *>(dy);
 #pragma unroll 4
             for (long long i = id; i < count / 4; i += threads) {
+                if (!in_array(4 * i + 3, count)) break;
                 const float4 v = q[i];
                 take(v.x), take(v.y), take(v.z), take(v.w);
             }
@@ -1065,7 +1086,8 @@ __global__ void __launch_bounds__(256) largest_kernel(const float *dy, long long
         for (long long i = done + id; i < count; i += threads) take(dy[i]);
     } else {
         for (long long r = id / 32; r < rows; r += threads / 32)
-            for (int c = lane; c < n; c += 32) take(dy[r * ld + c]);
+            for (int c = lane; c < n; c += 32)
+                if (in_array(r * ld + c, extent(rows, ld, n))) take(dy[r * ld + c]);
     }
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane == 0) sh[threadIdx.x >> 5] = m;
@@ -1090,6 +1112,7 @@ __global__ void __launch_bounds__(256) cast_colsum_kernel(const void *dy, long l
     float s = 0.f;
     if (c < n)
         for (long long r = r0 + ry; r < r1; r += 4) {
+            if (!in_array(r * ld + c, extent(rows, ld, n)) || (dst && !in_array(r * ld_dst + c, rows * ld_dst))) break;
             const float v = load_any(dy, r * ld + c, dy_type);
             if (dst) store_any(dst, r * ld_dst + c, dst_type, v * scale);
             s += v;
@@ -1115,12 +1138,14 @@ __global__ void __launch_bounds__(256) dz_kernel(const unsigned short *dy, long 
     if (c < n) {
 #pragma unroll 4
         for (long long r = blockIdx.y * rows_per_block + (threadIdx.x >> 3); r < r1; r += 32) {
+            if (!in_array(r * ld + c + 7, extent(rows, ld, n))) break;
             float v[8];
             unpack8(*reinterpret_cast<const uint4 *>(dy + r * ld + c), type, v);
             if constexpr (KEPT) {
+                const long long at = ((((r >> 7) * gridDim.x + blockIdx.x) * 4 + ((r >> 5) & 3)) * 8 + chunk) * 32 + (r & 31);
+                if (!in_array(at, kept_vectors(rows, n)) || !in_array(r * ld_dz + c + 7, rows * ld_dz)) break;
                 float d[8];
-                unpack8(kept[((((r >> 7) * gridDim.x + blockIdx.x) * 4 + ((r >> 5) & 3)) * 8 + chunk) * 32 + (r & 31)],
-                        QC_F16, d);
+                unpack8(kept[at], QC_F16, d);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] *= d[i] * (1.f / kKeptScale);
                 *reinterpret_cast<uint4 *>(dz + r * ld_dz + c) = pack8(v, type);
@@ -1161,13 +1186,14 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const float *part, int
     if (r < rows) {
 #pragma unroll 4
         for (int q = warp; q < splits; q += 8) {
+            if (!in_array(((long long)q * rows + r) * ld + c + 3, splits * rows * ld)) break;
             const float4 v = *reinterpret_cast<const float4 *>(part + ((long long)q * rows + r) * ld + c);
             s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
         }
     }
     sh[warp][lane] = s;
     __syncthreads();
-    if (warp || r >= rows) return;
+    if (warp || r >= rows || !in_array(r * n + min(c + 4, n) - 1, rows * n)) return;
 #pragma unroll
     for (int q = 1; q < 8; ++q) {
         const float4 v = sh[q][lane];
@@ -1549,7 +1575,9 @@ int ml_fault_word(unsigned int *word, int clear) {
         e = cudaMemcpyToSymbol(g_ml_fault_word, &zero, sizeof(zero));
     }
     QC_CUDA_TRY(e, "cudaMemcpyFromSymbol(fault word)");
-    *word = w;
+    unsigned int norm = 0;
+    if (int st = norm_fault_word(&norm, clear)) return st;
+    *word = w | norm;
     return 0;
 }
 
@@ -1693,7 +1721,7 @@ size_t linear_act_kept_bytes(long rows, int n, int k, int type, int out_type, in
     if (rows <= 512 || n < 8 || n % 8 || k < 512 || type != QC_BF16 || out_type != QC_BF16 || bias_type == QC_F32 ||
         activation <= QC_ACT_NONE || activation > QC_ACT_GELU || few_rows(rows, n, k, type))
         return 0;
-    return (size_t)((rows + 127) / 128) * ((n + 63) / 64) * (128 * 64 * 2);
+    return (size_t)kept_vectors(rows, n) * sizeof(uint4);
 }
 
 int linear_act_keep_cuda(const void *x, const void *weight, const void *bias, const void *residual, void *y, void *kept,

@@ -210,5 +210,8 @@ int launch_colsum_reduce(const float *partial, int parts, int n, void *out, int 
 
 bool aligned_to(const void *p, long long bytes);
 
+// The norms' fault word (the products' is ml_fault_word's own).
+int norm_fault_word(unsigned int *word, int clear);
+
 }  // namespace ml
 }  // namespace qc

@@ -30,9 +30,18 @@
 namespace qc {
 namespace ml {
 
+__device__ unsigned int g_norm_fault_word = 0;
+
 bool aligned_to(const void *p, long long bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 namespace {
+
+// Values first..last of an array of `total` (debug build; always true otherwise).
+__device__ __forceinline__ bool in_array(long long first, long long last, long long total) {
+    return QC_IN_BOUNDS(first, total, g_norm_fault_word) && QC_IN_BOUNDS(last, total, g_norm_fault_word);
+}
+// Values of rows of width n, ld apart.
+__device__ __forceinline__ long long extent(long long rows, long long ld, int n) { return (rows - 1) * ld + n; }
 
 struct NormArgs {
     const void *x, *res, *weight;
@@ -107,8 +116,13 @@ struct Span {
     // Columns c..c+V of a row at `at` in an array of `total` values. A partial
     // vector brings its neighbours' values along; mask() drops them, which
     // waits for the load, so all loads of a row are issued before.
+    // whether these columns of the row at `at` lie in an array of `total` values
+    __device__ __forceinline__ bool inside(long long at, int c, long long total) const {
+        return in_array(at + (SHIFT ? max(c, 0) : c), at + (SHIFT ? min(c + V, n) : c + V) - 1, total);
+    }
     template <int T>
     __device__ __forceinline__ void load(Raw<T, V> &r, const void *base, long long at, int c, long long total) const {
+        if (!inside(at, c, total)) return;
         if (!SHIFT || (at + c >= 0 && at + c + V <= total)) r.load(base, at + c);
         else r.load_some(base, at + c, -c, n - c);
     }
@@ -116,7 +130,9 @@ struct Span {
     __device__ __forceinline__ void mask(Raw<T, V> &r, int c) const {
         if (!whole(c)) r.keep(-c, n - c);
     }
-    __device__ __forceinline__ void store(void *base, long long at, int c, int type, const float (&v)[V]) const {
+    __device__ __forceinline__ void store(void *base, long long at, int c, int type, const float (&v)[V],
+                                          long long total) const {
+        if (!inside(at, c, total)) return;
         if (whole(c)) {
             store_vec<V>(base, at + c, type, v);
         } else {
@@ -142,14 +158,14 @@ __global__ void __launch_bounds__(L ? 256 : 512) rms_norm_kernel(NormArgs a) {
     // the first row of this warp's groups: loops end for whole warps together
     const long long first = kBlock ? group : group - (threadIdx.x % 32) / kL;
     const Span<V, SHIFT> span{a.n, SHIFT ? (int)(group % V * (a.n % V) % V) : 0};
-    const long long total_x = (a.rows - 1) * a.ldx + a.n, total_r = (a.rows - 1) * a.ldr + a.n;
+    const long long total_x = extent(a.rows, a.ldx, a.n), total_r = extent(a.rows, a.ldr, a.n);
 
     Raw<XT, V> w[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int c = span.col(j * lanes + lane);
         w[j].zero();
-        if (a.norm && span.any(c)) {
+        if (a.norm && span.any(c) && span.inside(0, c, a.n)) {
             if constexpr (SHIFT) w[j].load_some(a.weight, c, -c, a.n - c);
             else w[j].load(a.weight, c);
         }
@@ -234,7 +250,7 @@ __global__ void __launch_bounds__(L ? 256 : 512) rms_norm_kernel(NormArgs a) {
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
                     const int c = span.col(j * lanes + lane);
-                    if (row < a.rows && span.any(c)) span.store(a.h, row * a.n, c, XT, h[q][j]);
+                    if (row < a.rows && span.any(c)) span.store(a.h, row * a.n, c, XT, h[q][j], a.rows * a.n);
                 }
             }
             if (a.norm) {
@@ -270,12 +286,12 @@ __global__ void __launch_bounds__(L ? 256 : 512) rms_norm_kernel(NormArgs a) {
                             split(by(pair(h[q][j][i], h[q][j][i + 1])), h[q][j][i], h[q][j][i + 1]);
                     }
                 }
-                if (lane == 0 && row < a.rows) a.scale[row] = s;
+                if (lane == 0 && row < a.rows && in_array(row, row, a.rows)) a.scale[row] = s;
             }
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int c = span.col(j * lanes + lane);
-                if (row < a.rows && span.any(c)) span.store(a.y, row * a.n, c, a.out_type, h[q][j]);
+                if (row < a.rows && span.any(c)) span.store(a.y, row * a.n, c, a.out_type, h[q][j], a.rows * a.n);
             }
             // two uses of one slot array lie a barrier apart only when both
             // arrays are used (norm and scale); otherwise the block waits here
@@ -284,12 +300,24 @@ __global__ void __launch_bounds__(L ? 256 : 512) rms_norm_kernel(NormArgs a) {
     }
 }
 
+// Column c of a row in an array whose rows lie ld apart; in x, the residual and
+// the weight.
+template <typename Args>
+__device__ __forceinline__ bool in_rows(const Args &a, long long row, long long ld, int c) {
+    return in_array(row * ld + c, row * ld + c, extent(a.rows, ld, a.n));
+}
+template <typename Args>
+__device__ __forceinline__ bool at_inside(const Args &a, long long row, int c) {
+    return in_array(c, c, a.n) && in_rows(a, row, a.ldx, c) && (!a.res || in_rows(a, row, a.ldr, c));
+}
+
 // Rows of any width: one block per row, strided, read again for each pass.
 template <int XT>
 __global__ void __launch_bounds__(1024) rms_norm_wide_kernel(NormArgs a) {
     __shared__ float slots[2][32];
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         auto h_at = [&](int c) {
+            if (!at_inside(a, row, c)) return 0.f;
             float v = load_any(a.x, row * a.ldx + c, XT);
             if (a.res) v += load_any(a.res, row * a.ldr + c, XT);
             return v;
@@ -315,6 +343,7 @@ __global__ void __launch_bounds__(1024) rms_norm_wide_kernel(NormArgs a) {
             const float h = h_at(c);
             float y = a.norm ? h * r * load_any(a.weight, c, XT) : h;
             if (a.scale) y = Quotient(s)(y);
+            if (!in_array(row * a.n + c, row * a.n + c, a.rows * a.n)) continue;
             if (a.h) store_any(a.h, row * a.n + c, XT, h);
             store_any(a.y, row * a.n + c, a.out_type, y);
         }
@@ -330,6 +359,7 @@ struct NormGradArgs {
     long long rows, ldx, ldr, lddy, lddh;
     int n;
     float eps;
+    long long dw_room;  // values that dw_part has room for
 };
 
 template <int XT, int YT, int V, int L, int NV, int R, bool SHIFT>
@@ -345,7 +375,6 @@ __global__ void __launch_bounds__(L ? 256 : 512) rms_norm_grad_kernel(NormGradAr
     const long long groups = kBlock ? gridDim.x : (long long)gridDim.x * (blockDim.x / kL);
     const long long first = kBlock ? group : group - (threadIdx.x % 32) / kL;
     const Span<V, SHIFT> span{a.n, SHIFT ? (int)(group % V * (a.n % V) % V) : 0};
-    const long long last = a.rows - 1;
 
     Raw<XT, V> w[NV];
     float dw[NV][V];
@@ -353,7 +382,7 @@ __global__ void __launch_bounds__(L ? 256 : 512) rms_norm_grad_kernel(NormGradAr
     for (int j = 0; j < NV; ++j) {
         const int c = span.col(j * lanes + lane);
         w[j].zero();
-        if (span.any(c)) {
+        if (span.any(c) && span.inside(0, c, a.n)) {
             if constexpr (SHIFT) w[j].load_some(a.weight, c, -c, a.n - c);
             else w[j].load(a.weight, c);
         }
@@ -377,10 +406,10 @@ __global__ void __launch_bounds__(L ? 256 : 512) rms_norm_grad_kernel(NormGradAr
                 dy[q][j].zero();
                 dh[q][j].zero();
                 if (row < a.rows && span.any(c)) {
-                    span.load(x[q][j], a.x, row * a.ldx, c, last * a.ldx + a.n);
-                    if (a.res) span.load(res[q][j], a.res, row * a.ldr, c, last * a.ldr + a.n);
-                    span.load(dy[q][j], a.dy, row * a.lddy, c, last * a.lddy + a.n);
-                    if (a.dh) span.load(dh[q][j], a.dh, row * a.lddh, c, last * a.lddh + a.n);
+                    span.load(x[q][j], a.x, row * a.ldx, c, extent(a.rows, a.ldx, a.n));
+                    if (a.res) span.load(res[q][j], a.res, row * a.ldr, c, extent(a.rows, a.ldr, a.n));
+                    span.load(dy[q][j], a.dy, row * a.lddy, c, extent(a.rows, a.lddy, a.n));
+                    if (a.dh) span.load(dh[q][j], a.dh, row * a.lddh, c, extent(a.rows, a.lddh, a.n));
                 }
             }
 #pragma unroll
@@ -433,19 +462,23 @@ __global__ void __launch_bounds__(L ? 256 : 512) rms_norm_grad_kernel(NormGradAr
                     if (a.dh) dx[i] += dh[q][j].get(i);
                     if (row < a.rows) dw[j][i] += d * (hv * r);
                 }
-                if (a.dx && row < a.rows && span.any(c)) span.store(a.dx, row * a.n, c, XT, dx);
+                if (a.dx && row < a.rows && span.any(c)) span.store(a.dx, row * a.n, c, XT, dx, a.rows * a.n);
             }
         }
     }
     if (a.dw_part == nullptr) return;
     float *part = a.dw_part + (long long)blockIdx.x * a.n;
+    auto dw_inside = [&](int c) {
+        const long long at = gridDim.x == 1 ? c : (long long)blockIdx.x * a.n + c;
+        return in_array(at, at, gridDim.x == 1 ? a.n : a.dw_room);
+    };
     if constexpr (kBlock) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int c = span.col(j * lanes + lane) + i;
-                if (!span.holds(c)) continue;
+                if (!span.holds(c) || !dw_inside(c)) continue;
                 if (gridDim.x == 1) store_any(a.dw, c, XT, dw[j][i]);
                 else part[c] = dw[j][i];
             }
@@ -476,6 +509,7 @@ __global__ void __launch_bounds__(L ? 256 : 512) rms_norm_grad_kernel(NormGradAr
             __syncthreads();
         }
         for (int c = threadIdx.x; c < a.n; c += blockDim.x) {
+            if (!dw_inside(c)) continue;
             if (gridDim.x == 1) store_any(a.dw, c, XT, dw_sh[c]);
             else part[c] = dw_sh[c];
         }
@@ -489,10 +523,12 @@ __global__ void __launch_bounds__(1024) rms_norm_grad_wide_kernel(NormGradArgs a
     __shared__ float slots[2][32];
     float *part = a.dw_part ? a.dw_part + (long long)blockIdx.x * a.n : nullptr;
     auto h_at = [&](long long row, int c) {
+        if (!at_inside(a, row, c) || !in_rows(a, row, a.lddy, c) || (a.dh && !in_rows(a, row, a.lddh, c))) return 0.f;
         float v = load_any(a.x, row * a.ldx + c, XT);
         if (a.res) v += load_any(a.res, row * a.ldr + c, XT);
         return v;
     };
+    if (part && !in_array((long long)blockIdx.x * a.n, (long long)(blockIdx.x + 1) * a.n - 1, a.dw_room)) part = nullptr;
     if (part)
         for (int c = threadIdx.x; c < a.n; c += blockDim.x) part[c] = 0.f;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -510,7 +546,7 @@ __global__ void __launch_bounds__(1024) rms_norm_grad_wide_kernel(NormGradArgs a
             const float h = h_at(row, c), d = load_any(a.dy, row * a.lddy + c, YT);
             float dx = r * (d * load_any(a.weight, c, XT) - h * k);
             if (a.dh) dx += load_any(a.dh, row * a.lddh + c, XT);
-            if (a.dx) store_any(a.dx, row * a.n + c, XT, dx);
+            if (a.dx && in_array(row * a.n + c, row * a.n + c, a.rows * a.n)) store_any(a.dx, row * a.n + c, XT, dx);
             if (part) part[c] += d * (h * r);
         }
         __syncthreads();
@@ -527,6 +563,7 @@ __global__ void __launch_bounds__(256) colsum_reduce_kernel(const float *partial
     float s = 0.f;
     if (c < n) {
         int p = lane;
+        if (!QC_IN_BOUNDS(c, n, g_norm_fault_word)) p = parts;
         for (; p + 224 < parts; p += 256) {
             float v[8];
 #pragma unroll
@@ -732,6 +769,18 @@ int launch_colsum_reduce(const float *partial, int parts, int n, void *out, int 
     return 0;
 }
 
+int norm_fault_word(unsigned int *word, int clear) {
+    unsigned int w = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&w, g_norm_fault_word, sizeof(w));
+    if (e == cudaSuccess && clear) {
+        const unsigned int zero = 0;
+        e = cudaMemcpyToSymbol(g_norm_fault_word, &zero, sizeof(zero));
+    }
+    QC_CUDA_TRY(e, "cudaMemcpyFromSymbol(fault word)");
+    *word = w;
+    return 0;
+}
+
 }  // namespace ml
 }  // namespace qc
 
@@ -791,7 +840,8 @@ int rms_norm_grad_cuda(const void *x, const void *residual, const void *weight, 
     int parts = 0;
     if (rows > 0) {
         NormGradArgs a{x, residual, weight, dy, dh, dx, dweight ? static_cast<float *>(workspace) : nullptr, dweight,
-                       rows, x_stride, residual_stride, dy_stride, dh_stride, n, eps};
+                       rows, x_stride, residual_stride, dy_stride, dh_stride, n, eps,
+                       (long long)(workspace_bytes / sizeof(float))};
         int st = 0;
         const int key = x_type * 4 + dy_type;
         switch (key) {

@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import random
+import re
+from pathlib import Path
 
 import pytest
 
@@ -38,3 +40,19 @@ def test_parts_of_the_weight_gradient():
     assert _core.linear_act_form(3, 5000, 64, 64, _core.BF16, SMS)[2] == 9
     assert _core.linear_act_form(3, 200000, 64, 64, _core.BF16, SMS)[2] == 148
     assert _core.linear_act_form(3, 2**22, 4096, 4096, _core.BF16, SMS)[2] == 2**22 // 32768
+
+
+def test_decoder_kernels_check_their_indexes_in_the_debug_build():
+    """Every kernel that reads or writes global memory by itself goes through a
+    check; kernels are found by their __global__."""
+    csrc = Path(__file__).resolve().parents[1] / "quantem-cuda_b200" / "csrc"
+    for name in ("rms_norm.cu", "linear_act.cu"):
+        source = (csrc / name).read_text()
+        parts = re.split(r"^__global__ ", source, flags=re.M)[1:]
+        assert len(parts) >= 4
+        for part in parts:
+            body = part[: part.index("\n}\n")]
+            if re.match(r".*\bzero_kernel\b", body, flags=re.S):
+                continue  # its loop's condition is the bound
+            through = r"QC_IN_BOUNDS|in_array|in_rows|at_inside|inside\(|FewEpilogue|span\."
+            assert re.search(through, body), f"{name}: {body[:120]}"
