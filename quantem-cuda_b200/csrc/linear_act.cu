@@ -207,8 +207,11 @@ __device__ __forceinline__ void act_grad(float &z0, float &z1) {
 // Rows and columns that no 16-byte boundary divides leave by warp-wide plain
 // stores from the slab instead (and the residual comes in the same way).
 
-enum Epilogue { kForward = 0, kActGrad = 1, kPartial = 2, kForwardKeep = 3 };
+// kActGradScaled is a form of its own for its fp32 dy times S: in kActGrad, the
+// scale's branches alone cost 5 of 104 us on 262144 rows of 256 by 256 with GELU.
+enum Epilogue { kForward = 0, kActGrad = 1, kPartial = 2, kForwardKeep = 3, kActGradScaled = 4 };
 __host__ __device__ constexpr bool is_forward(int epi) { return epi == kForward || epi == kForwardKeep; }
+__host__ __device__ constexpr bool is_act_grad(int epi) { return epi == kActGrad || epi == kActGradScaled; }
 enum ResidualMode { kResNone = 0, kResTma = 1, kResWarp = 2, kResThread = 3 };
 
 // Division of 0 <= n < 2^31 by a fixed d: with 2^p >= 2^31 d and mul = ceil(2^p/d),
@@ -237,8 +240,8 @@ struct Product {
     void *y;  // plain-store outputs: contiguous [M, N]
     uint4 *kept;  // act'(z) kKeptScale in fp16: [row tile][64-column slab][quarter][8 columns][32 rows]
     void *colsum;  // [row tiles][N]: fp32 partial sums, or the sums themselves where there is one row tile
-    // The largest finite |dy| as bits, or null: the act grad pass stores dz S,
-    // the products of dz S are divided by S.
+    // The largest finite |dy| as bits, or null: kActGradScaled forms dz S (and
+    // divides its column sums by S), the products of dz S are divided by S.
     const unsigned int *dy_max;
     int colsum_type, bias_type, out_type, act, res_mode, tma_store;
 };
@@ -348,12 +351,13 @@ __device__ __forceinline__ uint4 pack8(const float *v, int type) {
 
 // 32 columns of one row: v holds the accumulators and leaves as what goes into
 // the slab. `chunk0`: the slab's first 16-byte chunk of these columns.
-template <int EPI, int ACT>
+// GRAD: a product of dz.
+template <int EPI, int ACT, bool GRAD>
 __device__ __forceinline__ void epilogue_32(const Product &p, float (&v)[32], unsigned char *slab, int row, int chunk0,
                                             const float *bias, const float *col_scale, float row_scale,
                                             const float *dy_row, int dy_left, uint4 *kept) {
     const bool wide = EPI == kPartial || p.out_type == QC_F32;
-    if constexpr (EPI == kForward || EPI == kPartial) {
+    if constexpr (GRAD) {
         if (p.dy_max) {
             const float s = gradient_scale<true>(*p.dy_max);
 #pragma unroll
@@ -404,10 +408,15 @@ __device__ __forceinline__ void epilogue_32(const Product &p, float (&v)[32], un
             }
         }
     }
-    if constexpr (EPI == kActGrad) {
+    if constexpr (is_act_grad(EPI)) {
 #pragma unroll
         for (int i = 0; i < 32; i += 2) act_grad<ACT>(v[i], v[i + 1]);
         if (p.res_mode == kResThread) {
+            if constexpr (EPI == kActGradScaled) {
+                const float s = gradient_scale<false>(*p.dy_max);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] *= s;
+            }
 #pragma unroll
             for (int i = 0; i < 32; ++i)
                 v[i] = i < dy_left && in_array(dy_row + i - static_cast<const float *>(p.res), extent(p.M, p.ld_res, p.N))
@@ -428,15 +437,6 @@ __device__ __forceinline__ void epilogue_32(const Product &p, float (&v)[32], un
         for (int c = 0; c < 8; ++c)
             *reinterpret_cast<float4 *>(slab + slab_at(row, chunk0 + c)) =
                 make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-    } else if (EPI == kActGrad && p.dy_max) {  // the column sums take v without S
-        const float s = gradient_scale<false>(*p.dy_max);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            float d[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = v[8 * c + i] * s;
-            *reinterpret_cast<uint4 *>(slab + slab_at(row, chunk0 + c)) = pack8(d, p.out_type);
-        }
     } else {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // g%2 + 2, ... of every second tile: while one pair of groups computes,
         // the other's loads and stores are under way (115 -> 107 us on 262144
         // rows of 256 by 256 with GELU; the forward, 65 us, takes 71 us so).
-        const bool in_turn = EPI != kActGrad || PAIR || slabs < 4;
+        const bool in_turn = !is_act_grad(EPI) || PAIR || slabs < 4;
         auto unit = [&](int j, int &it, int &slab) {
             if (!in_turn) {
                 it = (j >> (log_slabs - 1)) * 2 + (group >> 1);
@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int chunk0 = wide ? 0 : 4 * h;
                 const float *dy_row = nullptr;
                 int dy_left = 0;
-                if (EPI == kActGrad && p.res_mode == kResThread && m0 + row < p.M) {
+                if (is_act_grad(EPI) && p.res_mode == kResThread && m0 + row < p.M) {
                     dy_row = static_cast<const float *>(p.res) + (m0 + row) * p.ld_res + c0;
                     dy_left = p.N - c0;
                 }
@@ -717,23 +717,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     kept = p.kept + ((((long long)m * ((p.N + 63) / 64) + col0 / 64) * 4 + quarter) * 8 + 4 * h) * 32 + lane;
                 switch (EPI == kPartial ? QC_ACT_NONE : p.act) {
                     case QC_ACT_RELU:
-                        epilogue_32<EPI, QC_ACT_RELU>(p, v, buf, row, chunk0, b, cs, row_scale, dy_row, dy_left,
+                        epilogue_32<EPI, QC_ACT_RELU, B_MN>(p, v, buf, row, chunk0, b, cs, row_scale, dy_row, dy_left,
                                                       kept);
                         break;
                     case QC_ACT_SILU:
-                        epilogue_32<EPI, QC_ACT_SILU>(p, v, buf, row, chunk0, b, cs, row_scale, dy_row, dy_left,
+                        epilogue_32<EPI, QC_ACT_SILU, B_MN>(p, v, buf, row, chunk0, b, cs, row_scale, dy_row, dy_left,
                                                       kept);
                         break;
                     case QC_ACT_GELU:
-                        epilogue_32<EPI, QC_ACT_GELU>(p, v, buf, row, chunk0, b, cs, row_scale, dy_row, dy_left,
+                        epilogue_32<EPI, QC_ACT_GELU, B_MN>(p, v, buf, row, chunk0, b, cs, row_scale, dy_row, dy_left,
                                                       kept);
                         break;
                     default:
-                        epilogue_32<EPI, QC_ACT_NONE>(p, v, buf, row, chunk0, b, cs, row_scale, dy_row, dy_left,
+                        epilogue_32<EPI, QC_ACT_NONE, B_MN>(p, v, buf, row, chunk0, b, cs, row_scale, dy_row, dy_left,
                                                       kept);
                         break;
                 }
-                if constexpr (EPI == kActGrad) {
+                if constexpr (is_act_grad(EPI)) {
                     if (p.colsum) {
                         // rows past the last hold the bias's z times a zero dy
                         if (m0 + row >= p.M) {
@@ -761,13 +761,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         fetch(j + 1);
                     }
                 }
-                if constexpr (EPI == kActGrad) {
+                if constexpr (is_act_grad(EPI)) {
                     const int c = (ew & 3) * 32 + lane;
                     if (p.colsum && c < 64 && col0 + c < p.N && m0 < p.M &&
                         in_array((long long)m * p.N + col0 + c, (p.M + 127) / 128 * p.N)) {
                         const float *cs = &sm.colsum[group][j & 1][0][c];
-                        store_any(p.colsum, (long long)m * p.N + col0 + c, p.colsum_type,
-                                  (cs[0] + cs[64]) + (cs[128] + cs[192]));
+                        float sum = (cs[0] + cs[64]) + (cs[128] + cs[192]);
+                        if constexpr (EPI == kActGradScaled) sum *= gradient_scale<true>(*p.dy_max);
+                        store_any(p.colsum, (long long)m * p.N + col0 + c, p.colsum_type, sum);
                     }
                 }
                 __syncwarp();
@@ -1828,7 +1829,8 @@ static int backward(const char *fn, const void *x, const void *weight, const voi
         if (int st = make_map(&map_y, ws + g.at_dz, type, n, rows, g.ld_dz, 128, 3)) return st;
         if (p.res_mode == kResTma)
             if (int st = make_map(&map_r, dy, type, n, rows, dy_stride, 128, 3)) return st;
-        if (int st = run_product<false, false, false, kActGrad>(xo, wo, type, k, map_y, map_r, p, sms, dev, stream))
+        if (int st = dy_max ? run_product<false, false, false, kActGradScaled>(xo, wo, type, k, map_y, map_r, p, sms, dev, stream)
+                            : run_product<false, false, false, kActGrad>(xo, wo, type, k, map_y, map_r, p, sms, dev, stream))
             return st;
         dzo = {ws + g.at_dz, g.ld_dz};
     } else if (g.vectors && (kept || sums)) {
