@@ -290,7 +290,7 @@ struct ProductSmem {
 // Waits for a phase of `bar`, for 2 s at most; a wait that gives up sets the
 // fault word and `gave_up`, after which no wait of the CTA lingers. The
 // epilogue then runs through its remaining slabs (so that every thread meets
-// every barrier) and the kernel ends with the fault word set.
+// every barrier), fills them with NaN, and the kernel ends with the fault word set.
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *gave_up) {
     if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = global_timer_ns();
@@ -305,9 +305,12 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile in
     return true;
 }
 // Waits for copies or products still in flight before the CTA leaves.
-__device__ __forceinline__ void drain(uint64_t *bar, uint32_t parity) {
-    if (!mbar_wait_bounded(bar, parity, kWaitLimitNs)) atomicOr(&g_ml_fault_word, QC_FAULT_TMA_WAIT);
+__device__ __forceinline__ bool drain(uint64_t *bar, uint32_t parity) {
+    if (mbar_wait_bounded(bar, parity, kWaitLimitNs)) return true;
+    atomicOr(&g_ml_fault_word, QC_FAULT_TMA_WAIT);
+    return false;
 }
+constexpr uint32_t kNaNBits = 0xffffffffu;  // two NaN in 16 bits
 
 // Tiles go to the CTAs (pairs) in groups of 2048 rows, rows fastest, so that the
 // tiles in flight share rows of A and of B in L2. m counts 128 or 256 rows.
@@ -600,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                           k > k0 || j > 0);
                     tc::mma_commit<PAIR>(&sm.empty[st]);
                 }
-                tc::mma_commit<PAIR>(&sm.acc_full[acc]);
+                if (ok) tc::mma_commit<PAIR>(&sm.acc_full[acc]);  // else the epilogue's wait gives up too
             }
             // the last products have finished reading the ring: the final
             // commits' barriers complete only then
@@ -666,6 +669,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (EPI != kPartial) look_ahead(0);
 
         int it, slab;
+        bool sound = true;  // no wait of this thread has given up (a later phase of the same parity says nothing)
         for (int j = 0; unit(j, it, slab); ++j) {
             int m, n, s;
             tile_of<PAIR>(p, first_tile + it * tile_step, m, n, s);
@@ -694,8 +698,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (EPI != kPartial && p.res_mode == kResWarp)
                 slab_warp_copy<true>(p, buf, const_cast<void *>(p.res), p.ld_res, m0, row0, col0, lane);
             __syncwarp();
-            if (tma_res) wait(&sm.res_full[group], j & 1, &sm.gave_up);
-            wait(&sm.acc_full[it % A], (it / A) & 1, &sm.gave_up);
+            if (tma_res) sound = wait(&sm.res_full[group], j & 1, &sm.gave_up) && sound;
+            sound = wait(&sm.acc_full[it % A], (it / A) & 1, &sm.gave_up) && sound;
             __syncwarp();
             tc::fence_after();
             const uint32_t acc = tmem + it % A * BN + slab * slab_cols + ((uint32_t)row0 << 16);
@@ -740,9 +744,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = 0.f;
                         }
-                        sm.colsum[group][j & 1][ew & 3][32 * h + lane] = column_sums(v, lane);
+                        const float sum = column_sums(v, lane);
+                        sm.colsum[group][j & 1][ew & 3][32 * h + lane] = sound ? sum : __uint_as_float(kNaNBits);
                     }
                 }
+            }
+            if (!sound) {
+                for (int c = 0; c < 8; ++c)
+                    *reinterpret_cast<uint4 *>(buf + row * 128 + 16 * c) = make_uint4(kNaNBits, kNaNBits, kNaNBits, kNaNBits);
             }
             tc::fence_before();
             __syncwarp();
@@ -814,6 +823,12 @@ struct FewSmem {
     int gave_up;
 };
 
+__device__ __forceinline__ void spoil(float (&v)[16], bool sound) {
+    if (sound) return;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(kNaNBits);
+}
+
 // One column (feature) per lane, eight rows of x at a time, straight-line code:
 // with one warp per scheduler the latencies must overlap within the thread.
 template <int ACT, int OT>
@@ -853,10 +868,11 @@ struct FewEpilogue {
     }
 
     // the whole reduction lies in this CTA: from the accumulator
-    __device__ __forceinline__ void whole(uint32_t acc, int cols) const {
+    __device__ __forceinline__ void whole(uint32_t acc, int cols, bool sound) const {
         for (int c = 0; c < cols; c += 16) {
             float v[16], z[8];
             tc::tmem_load_16(acc + c, v);
+            spoil(v, sound);
 #pragma unroll
             for (int h = 0; h < 16; h += 8) {
 #pragma unroll
@@ -957,9 +973,10 @@ __global__ void __launch_bounds__(192, 1)
     } else if (warp == 1) {
         if (lane == 0) {
             int q = 0;
+            bool ok = true;
             for (int k = k0; k < k1; ++k, ++q) {
                 const int st = q % S;
-                if (!wait(&sm.full[st], (q / S) & 1, &sm.gave_up)) break;
+                if (!(ok = wait(&sm.full[st], (q / S) & 1, &sm.gave_up))) break;
                 tc::fence_after();
                 const uint32_t a = smem_addr(sm.ring[st]);
                 const uint64_t da = tc::operand_desc(a, 16), db = tc::operand_desc(a + kStageA, 16);
@@ -967,12 +984,13 @@ __global__ void __launch_bounds__(192, 1)
                 for (int j = 0; j < 4; ++j) tc::mma<F8>(tmem, da + 2 * j, db + 2 * j, p.idesc, k > k0 || j > 0);
                 tc::mma_commit(&sm.empty[st]);
             }
-            tc::mma_commit(&sm.done);
+            if (ok) tc::mma_commit(&sm.done);
         }
         __syncwarp();
     }
-    // every thread: all products are done, the ring is free
-    drain(&sm.done, 0);
+    // every thread: all products are done, the ring is free (a wait that gave up
+    // leaves NaN)
+    const bool sound = drain(&sm.done, 0);
     tc::fence_after();
     __syncthreads();
     float *part = reinterpret_cast<float *>(sm.ring);
@@ -987,7 +1005,7 @@ __global__ void __launch_bounds__(192, 1)
     if (parts == 1) {
         if (warp >= 2) {
             with_act_and_type(p.act, p.out_type, [&](auto act, auto type) {
-                FewEpilogue<decltype(act)::value, decltype(type)::value>{p, r0, f, b, cs}.whole(acc, cols);
+                FewEpilogue<decltype(act)::value, decltype(type)::value>{p, r0, f, b, cs}.whole(acc, cols, sound);
             });
             tc::fence_before();
         }
@@ -1000,6 +1018,7 @@ __global__ void __launch_bounds__(192, 1)
         for (int c = 0; c < cols; c += 16) {
             float v[16];
             tc::tmem_load_16(acc + c, v);
+            spoil(v, sound);
 #pragma unroll
             for (int i = 0; i < 16; ++i) part[(c + i) * 128 + f_local] = v[i];
         }
