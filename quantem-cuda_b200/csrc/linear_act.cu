@@ -32,7 +32,6 @@
 // are applied to the fp32 value, which is rounded once.
 #include <algorithm>
 #include <atomic>
-#include <mutex>
 #include <type_traits>
 
 #include "ml_common.cuh"
@@ -1233,27 +1232,6 @@ __global__ void __launch_bounds__(256) zero_kernel(unsigned char *p, long long b
 
 // ── host side ────────────────────────────────────────────────────────────
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-int get_encode_fn(EncodeTiledFn *fn) {
-    static std::once_flag once;
-    static EncodeTiledFn cached = nullptr;
-    static cudaError_t err = cudaSuccess;
-    static cudaDriverEntryPointQueryResult qres = cudaDriverEntryPointSuccess;
-    std::call_once(once, [] {
-        void *p = nullptr;
-        err = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres);
-        cached = reinterpret_cast<EncodeTiledFn>(p);
-    });
-    if (err != cudaSuccess) return check_cuda(err, "cudaGetDriverEntryPoint(cuTensorMapEncodeTiled)");
-    if (cached == nullptr || qres != cudaDriverEntryPointSuccess)
-        return set_error(QC_ERR_NO_DEVICE, "cuTensorMapEncodeTiled is not available from the driver");
-    *fn = cached;
-    return 0;
-}
-
 CUtensorMapDataType map_type(int t) {
     switch (t) {
         case QC_F32: return CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
@@ -1268,7 +1246,7 @@ CUtensorMapDataType map_type(int t) {
 int make_map(CUtensorMap *map, const void *base, int type, long long cols, long long rows, long long ld, int box_rows,
              int dims, long long planes = 1) {
     EncodeTiledFn encode = nullptr;
-    if (int st = get_encode_fn(&encode)) return st;
+    if (int st = tensor_map_encoder(&encode)) return st;
     const int es = elem_size(type);
     const cuuint64_t size[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
     const cuuint64_t pitch[2] = {(cuuint64_t)(ld * es), (cuuint64_t)(ld * es * rows)};

@@ -38,6 +38,12 @@ int check_cuda(cudaError_t err, const char *what);
 int device_sm_count(int *sms);
 int device_sm_count(int dev, int *sms);
 
+// The driver's cuTensorMapEncodeTiled (the library links no libcuda).
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int tensor_map_encoder(EncodeTiledFn *fn);
+
 // NVTX range over a C-ABI entry point, so that a profiler timeline shows each
 // call by name next to its kernels (NVTX costs nothing without a tool).
 struct NvtxRange {

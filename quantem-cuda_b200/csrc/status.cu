@@ -58,6 +58,23 @@ int device_sm_count(int dev, int *sms) {
     return 0;
 }
 
+int tensor_map_encoder(EncodeTiledFn *fn) {
+    static std::once_flag once;
+    static EncodeTiledFn cached = nullptr;
+    static cudaError_t err = cudaSuccess;
+    static cudaDriverEntryPointQueryResult qres = cudaDriverEntryPointSuccess;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        err = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres);
+        cached = reinterpret_cast<EncodeTiledFn>(p);
+    });
+    if (err != cudaSuccess) return check_cuda(err, "cudaGetDriverEntryPoint(cuTensorMapEncodeTiled)");
+    if (cached == nullptr || qres != cudaDriverEntryPointSuccess)
+        return set_error(QC_ERR_NO_DEVICE, "cuTensorMapEncodeTiled is not available from the driver");
+    *fn = cached;
+    return 0;
+}
+
 }  // namespace qc
 
 extern "C" {

@@ -1347,28 +1347,6 @@ __global__ void __launch_bounds__(kFinThreads) tv_finalize_peer_kernel(const Fin
 
 // ── host side ────────────────────────────────────────────────────────────
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
-                                  const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-int get_encode_fn(EncodeTiledFn *fn) {
-    static std::once_flag once;
-    static EncodeTiledFn cached = nullptr;
-    static cudaError_t err = cudaSuccess;
-    static cudaDriverEntryPointQueryResult qres = cudaDriverEntryPointSuccess;
-    std::call_once(once, [] {
-        void *p = nullptr;
-        err = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres);
-        cached = reinterpret_cast<EncodeTiledFn>(p);
-    });
-    if (err != cudaSuccess) return check_cuda(err, "cudaGetDriverEntryPoint(cuTensorMapEncodeTiled)");
-    if (cached == nullptr || qres != cudaDriverEntryPointSuccess)
-        return set_error(QC_ERR_NO_DEVICE, "cuTensorMapEncodeTiled is not available from the driver");
-    *fn = cached;
-    return 0;
-}
-
 // Chooses the D-chunk of the chunk-major units. Each CTA runs its units one
 // after another, so the time is modelled as rounds × (chunk + halo planes),
 // rounds = ceil(units / resident CTAs); ties go to the larger chunk (fewer
@@ -1438,7 +1416,7 @@ int launch_variant(bool use_tma, const float *vol, const float *g, float *grad, 
         using G = typename std::conditional<is_mix(V), typename MixGeom<V>::type,
                                             typename FastGeomFor<V>::type>::type;
         EncodeTiledFn encode = nullptr;
-        if (int st = get_encode_fn(&encode)) return st;
+        if (int st = tensor_map_encoder(&encode)) return st;
         // The tensor map is encoded through the driver API, which needs a
         // current context on this thread; a thread that has made no runtime
         // call yet (autograd's backward thread, a fresh host thread) has none.
