@@ -504,12 +504,17 @@ int linear_act_cuda(const void *x, const void *weight, const void *bias, const v
 #define QC_PRODUCT_DWEIGHT 3
 int linear_act_form(int product, long rows, int n, int k, int type, int sms, int *form);
 
+/* A wait of a product's kernel for its own copies or products that runs out (2 s)
+ * sets QC_FAULT_TMA_WAIT in the device's fault word; what depends on it is NaN. */
+
 /* Backward of linear_act for 16-bit operands: dx[rows, k] and dweight[n, k] of
  * `type`, dbias[n] of bias_type, each written if not NULL (the residual's
  * gradient is dy). dy has `type` or QC_F32; dz = dy activation'(z) is rounded to
  * `type` for the products (QC_F16 from QC_F32: scaled by a power of two that brings
  * the largest |dy| near fp16's). Sums over rows are taken in a fixed order. The
- * workspace's size depends on the same arguments and on the device. */
+ * workspace's size depends on the same arguments and on the device: dz, and
+ * dweight's partial sums, 4 n k bytes per part of the rows (linear_act_form's
+ * QC_PRODUCT_DWEIGHT; 2 GB for a million rows of 4096 by 4096). */
 size_t linear_act_grad_workspace_bytes(const void *x, const void *weight, const void *dy, const void *dx,
                                        const void *dweight, const void *dbias, long rows, int n, int k, long x_stride,
                                        long weight_stride, long dy_stride, int type, int dy_type, int activation,

@@ -11,15 +11,19 @@
 // lie, no transposed copy is made.
 //
 // The backward needs dz = dy act'(z), in 16 bits as the next products' operand
-// (at most half a step of its type off), and its column sums, taken in fp32
-// before that rounding. Two ways to it:
+// (at most half a step of its type off: dx and dW, themselves rounded to 16 bits,
+// come out 1.4 times as far from their 64-bit values as from an unrounded dz; two
+// 16-bit parts of dz would take that away at twice the work of both products), and
+// its column sums, taken in fp32 before that rounding. Two ways to it:
 // * z is formed again from x and W, and the epilogue multiplies dy by act'(z):
 //   nothing is kept, nothing rounded but dz;
 // * a large bf16 forward keeps act'(z) itself, which lies within [-0.13, 1.13],
 //   in fp16 times 2^12: at most half a step off, 2^-11 of its value (an eighth of
 //   dz's own rounding) down to 2^-26, and 2^-37 below; z in 16 bits would add as
-//   much as dz's rounding. A pass over dy then gives dz (8192 rows of 1024 by
-//   4096, SiLU: 44 us, against 80 us).
+//   much as dz's rounding. A pass over dy then gives dz. A training pass of 8192
+//   rows of 1024 by 4096 (SiLU) takes 253 us so and 290 us with z formed again,
+//   32768 rows of 512 by 512 121 and 134 us, 16384 of 2048 by 2048 413 and 501 us
+//   (loops of a second in turn).
 //
 // fp16 has too few exponents for fp32 upstream gradients (a loss averaged over
 // many values, a scaled one): there dz is multiplied by a power of two S that
@@ -75,9 +79,9 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // Forward: Phi(z) = 1/(1 + exp(-g(z))), g the log odds. g(z)/z is an even,
 // smooth function: a polynomial of degree 7 in u = z^2 <= 30, fitted by the
 // Lawson iteration (least squares, reweighted towards the least largest error)
-// so that z Phi(z) is within 7.8e-8, and within 1.4e-3 of its own value in the
-// far negative tail, where it is below 1e-6. Coefficients are scaled by
-// -1/ln 2. One exponential and one reciprocal per value, no selection by sign.
+// so that z Phi(z) is within 7.8e-8, and within 1.4e-3 of its own value as far as
+// z = -5.47. Beyond, where it is below 1.3e-7, the absolute bound alone holds (4
+// times the value at -6, 125 times at -7). Coefficients are scaled by -1/ln 2. One exponential and one reciprocal per value, no selection by sign.
 // KEEP: the derivative Phi(z) + z phi(z) too, to d.
 template <bool KEEP = false>
 __device__ __forceinline__ void gelu(float &z0, float &z1, float *d = nullptr) {
@@ -202,7 +206,7 @@ __device__ __forceinline__ void act_grad(float &z0, float &z1) {
 // 128 rows of A and half of B's rows, and the leading CTA's matrix instructions
 // read both halves: a CTA fetches 32 KB instead of 48 KB per 128 x 256 x 64
 // products, which is what long reductions are bound by (16384 x 4096 x 4096 in
-// bf16: 428 us, single CTAs 488 us).
+// bf16: 428 us, single CTAs 488 us, cold; 467 us in a loop of seconds).
 // Rows and columns that no 16-byte boundary divides leave by warp-wide plain
 // stores from the slab instead (and the residual comes in the same way).
 
@@ -1712,9 +1716,9 @@ int linear_act_cuda(const void *x, const void *weight, const void *bias, const v
 }
 
 // Where keeping act'(z) pays: large bf16 products with an activation and a reduction
-// of 512 or more (of 1024: 228 against 255 us for a training pass of 8192 rows; of
-// 256: 292 against 296 us, not worth the memory). fp16 dz has too few bits less to
-// hide the rounding, and an fp32 bias gradient would show it.
+// of 512 or more (the file's head has times; of 256, 262144 rows: 292 against 296
+// us, not worth the memory). fp16 dz has too few bits less to hide the rounding, and
+// an fp32 bias gradient would show it.
 size_t linear_act_kept_bytes(long rows, int n, int k, int type, int out_type, int bias_type, int activation) {
     if (rows <= 512 || n < 8 || n % 8 || k < 512 || type != QC_BF16 || out_type != QC_BF16 || bias_type == QC_F32 ||
         activation <= QC_ACT_NONE || activation > QC_ACT_GELU || few_rows(rows, n, k, type))

@@ -56,7 +56,7 @@ constexpr float kE4M3Max = 448.f;
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126
 
 // Division by a scale of at least 2^-126: the product with its reciprocal and one
-// correction, which rounds like the quotient itself; the product alone moves
+// correction by the remainder (Markstein, 1990), which rounds like the quotient itself; the product alone moves
 // values across the borders of e4m3's steps twice as often. An infinite scale
 // takes finite values to 0 and the infinite one to NaN, as division does.
 struct Quotient {

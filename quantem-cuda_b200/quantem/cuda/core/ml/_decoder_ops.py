@@ -341,7 +341,7 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6, out_dtype: torch.dtyp
 
         y = x / sqrt(mean(x**2) + eps) * weight
 
-    Differentiable w.r.t. ``x`` and ``weight``. Sums are fp32; ``y`` is rounded
+    Differentiable w.r.t. ``x`` and ``weight`` (in reverse mode). Sums are fp32; ``y`` is rounded
     once. Gradients are the same from run to run.
 
     Args:
@@ -364,9 +364,9 @@ def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float = 1e-6,
         y = h / sqrt(mean(h**2) + eps) * weight
 
     Returns ``(y, h)``; ``h`` has x's type and is the next residual. ``y`` and
-    the gradients are formed from the unrounded sum. The gradients of ``x`` and ``residual`` are one tensor. ``residual`` has x's
-    shape and type (an expanded one is read in place). Otherwise as
-    :func:`rms_norm`.
+    the gradients are formed from the unrounded sum. The gradients of ``x`` and
+    ``residual`` are one tensor. ``residual`` has x's shape and type (an expanded
+    one is read in place). Otherwise as :func:`rms_norm`.
     """
     if residual is None:
         raise TypeError("add_rms_norm: residual is missing (rms_norm norms x alone)")
@@ -640,7 +640,9 @@ def linear_act(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual: 
     derivative instead (2 bytes per output until the backward). It rounds
     dz = dy activation'(z) to x's type before the products with weight and x; fp32
     gradients of fp16 calls are scaled by a power of two for it (dz below 2**-39
-    of the largest dy is lost), fp16 ones beyond 57000 may overflow. Products
+    of the largest dy is lost), fp16 ones beyond 57000 may overflow. Its
+    workspace holds dz and partial sums of weight's gradient (2 GB for a million
+    rows of 4096 by 4096). No forward-mode derivative. Products
     run on the tensor cores with fp32 accumulation, the epilogue is fp32, and
     ``y`` is rounded once. Sums over rows are taken in a fixed order: outputs
     and gradients are the same from run to run.
