@@ -116,6 +116,7 @@ struct Arg {
             count *= size[i];
         }
         ptr = (uintptr_t)call_int(o, names.data_ptr);
+        require(ptr != 0 || count == 0);  // torch.func's tensors have no address of their own
     }
     bool given() const { return o != nullptr; }
     long long last() const { return size[dims - 1]; }

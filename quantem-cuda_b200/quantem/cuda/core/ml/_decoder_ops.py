@@ -14,8 +14,8 @@ bits (e4m3 with scales) for serving.
 The features come as fp32 ``[points, T*C]``; the norm's ``out_dtype`` takes
 them to the decoder's type. As in the K-Planes layer, the public wrappers call
 the implementations directly when they run eagerly, and the registered ops
-while a graph is recorded (``torch.compile``, ``make_fx``, ``torch.jit.trace``)
-and for tensor subclasses. Forward-mode derivatives are refused.
+while a graph is recorded (``torch.compile``, ``make_fx``, ``torch.jit.trace``),
+inside ``torch.func`` transforms and for tensor subclasses. Forward-mode derivatives are refused.
 """
 
 from __future__ import annotations
@@ -46,14 +46,16 @@ _core.decoder_setup(Tensor, torch.nn.Parameter, (torch.float32, torch.bfloat16, 
 _is_compiling = torch.compiler.is_compiling
 _early_modes = torch._ops._len_torch_dispatch_stack_pre_dispatch
 _trace = torch._C._get_tracing_state
+_transform = torch._C._functorch.maybe_current_level
 
 
 def _direct() -> bool:
     """Whether a call may pass torch's dispatcher by. Not while a graph is
     recorded, which would hold the outputs' allocations alone; not inside a
-    forward-mode level, whose tangents those allocations would drop."""
+    forward-mode level, whose tangents those allocations would drop; not inside
+    a torch.func transform, whose tensors may have no address."""
     return not (_is_compiling() or forward_ad._current_level >= 0 or _dispatch_modes() or _early_modes()
-                or _trace() is not None)
+                or _trace() is not None or _transform() is not None)
 
 
 def _no_forward_mode(fn: str, *tensors: Tensor | None) -> None:
@@ -322,7 +324,7 @@ def _norm_call(fn: str, x: Tensor, residual: Tensor | None, weight: Tensor, eps:
     eps = float(eps)
     if out_dtype is not _FP8 and not _is_compiling():
         outs = _core.decoder_norm(x, residual, weight, eps, out_dtype, True)
-        if outs is None and _trace() is None:  # plain tensors, a gradient is recorded
+        if outs is None and _direct():  # plain tensors, a gradient is recorded
             return _RmsNorm.apply(fn, x, residual, weight, eps, out_dtype)
         if outs is not NotImplemented and outs is not None:
             return outs
@@ -661,7 +663,7 @@ def linear_act(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual: 
     """
     if not _is_compiling():
         y = _core.decoder_linear(x, weight, bias, residual, None, None, activation, out_dtype, True)
-        if y is None and _trace() is None:  # plain tensors, a gradient is recorded
+        if y is None and _direct():  # plain tensors, a gradient is recorded
             return _LinearAct.apply(x, weight, bias, residual, activation, out_dtype)
         if y is not NotImplemented and y is not None:
             return y

@@ -7,6 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch.func import functionalize
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from quantem.cuda.core import ml
@@ -112,3 +113,34 @@ def test_backward_recorded_apart_from_its_forward():
         assert any("quantem_cuda" in str(n.target) for n in graph.graph.nodes)
         for got, ref in zip(graph(2 * dy), want):
             assert (got.float() - 2 * ref.float()).norm() <= 2.0**-6 * ref.float().norm()
+
+
+def test_transformed_tensors():
+    """torch.func wraps its tensors: their address is null or cannot be asked
+    for. None is taken for a missing argument; torch.func's own gradients and vmap
+    are refused."""
+    x, w, nw = _inputs()
+    b, r = w[:, 0].contiguous(), torch.randn(40, 72, device="cuda").to(BF16)
+    want = ml.linear_act(x, w, b, r, "silu")
+    assert torch.equal(functionalize(lambda t: ml.linear_act(x, w, t, r, "silu"))(b), want)
+    assert torch.equal(functionalize(lambda t: ml.linear_act(x, w, b, t, "silu"))(r), want)
+    assert torch.equal(functionalize(lambda t: ml.linear_act(t, w, b, r, "silu"))(x), want)
+    want = ml.add_rms_norm(x, x, nw)
+    for got in (functionalize(lambda t: ml.add_rms_norm(x, t, nw))(x), functionalize(lambda t: ml.add_rms_norm(x, x, t))(nw)):
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+    def loss(t):
+        return ml.linear_act(ml.rms_norm(t, nw), w, b, activation="gelu", out_dtype=F32).square().sum()
+
+    with pytest.raises(RuntimeError, match="functorch transforms"):
+        torch.func.grad(loss)(x)
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda t: ml.rms_norm(t, nw))(x)
+
+
+def test_calls_under_a_function_mode():
+    """torch.device as a context is one; the values are the same."""
+    a = _inputs()
+    want = _chain(*a)
+    with torch.device("cuda"):
+        assert torch.equal(_chain(*a), want)

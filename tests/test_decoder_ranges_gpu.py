@@ -185,3 +185,33 @@ def test_scales_whose_product_leaves_fp32(rows):
     zero = torch.zeros(rows, k, device="cuda").to(E4M3)
     y = ml.linear_act_fp8(zero, torch.full_like(sx, 1e25), w, torch.full_like(sw, 1e20), out_dtype=F32)
     assert not y.any()
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_scaled_gradients_in_a_graph(act):
+    """The scale is formed on the device: a captured backward follows the
+    gradients that it is replayed on. On another stream, too."""
+    g = _gen(13)
+    x, w = _randn(g, 700, 64).to(F16).requires_grad_(), _randn(g, 48, 64).to(F16).requires_grad_()
+    dy = _randn(g, 700, 48)
+
+    def step():
+        return torch.autograd.grad(ml.linear_act(x, w, activation=act, out_dtype=F32), [x, w], dy)
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    del got
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for size in (1.0, 2.0**-20, 2.0**14, 2.0**-30):
+        dy.copy_(_randn(g, 700, 48, scale=size))
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, outs))
